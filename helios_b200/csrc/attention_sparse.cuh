@@ -1,0 +1,520 @@
+// Decode attention over the key blocks that a cheap score selects for each query.
+//
+// Keys are taken in blocks of 64. For each block and KV head the pool keeps the elementwise
+// minimum lo and maximum hi of its keys (key_block_bounds_kernel). For a query q,
+//   sum_d max(q_d lo_d, q_d hi_d) = sum_d min(q_d, 0) lo_d + max(q_d, 0) hi_d
+// is at least q . k for every key of the block. A block's score is the largest of these over
+// the query heads that share the KV head; of a row's blocks the first `sink` and the last
+// `recent` are always taken, then those with the largest scores (equal scores: the lower block;
+// NaN counts as the largest, so a damaged block shows in the output) up to `top` in all. The
+// output is softmax attention over the keys of these blocks alone.
+//
+// The right-hand form is a product over 256 dims, [min(q, 0) | max(q, 0)] . [lo | hi], so the
+// scores of all heads of a group come from m16n8k16 MMAs (heads as M, blocks as N) at the cost
+// of reading the bounds: 512 bytes per block where the block's K and V are 32 KB. Their fp32
+// error is at most eps = 2^-15 sum |terms| (256 exact products, each addition rounded or
+// truncated at 2^-23 or better). Blocks further than 2 eps from the threshold, the k-th largest
+// computed score, are settled by it; the few within are scored again in 64 bits, where 256
+// products of two 8-bit significands sum exactly or very nearly so, and ranked by that. The
+// selection is therefore that of exact scores.
+#pragma once
+
+#include "attention_decode.cuh"
+#include "linear_w4.cuh"
+
+namespace hb {
+
+constexpr int kBlockKeys = kDecTileKeys;  // keys per block: one tile of the decode ring
+
+// ---------------------------------------------------------------- bounds
+struct BlockBoundsParams {
+  const __nv_bfloat16* keys;  // [num_pages, page_size, kv_heads, 128]
+  __nv_bfloat16* bounds;      // [num_pages, kv_heads, page_size / 64, 2, 128]
+  const int32_t* block_table;  // [rows, width]
+  const int32_t* cu_seq_q;     // [rows + 1]
+  const int32_t* seqused_k;    // [rows]
+  const int32_t* token_row;    // [tokens]
+  int32_t rows, tokens, width, num_pages, page_size, kv_heads;
+};
+
+constexpr int kBoundsThreads = 256;
+
+// One CTA per token of the tick; the CTA of the first token that a row has in a block (in this
+// tick) computes the block's bounds anew from the pool, over the keys the row has there by now.
+// Nothing is carried over from earlier bounds, so truncated and rewritten keys leave no trace.
+// A warp takes a KV head's keys: 8 bytes per lane, a 256-byte row per load.
+__global__ void __launch_bounds__(kBoundsThreads) key_block_bounds_kernel(BlockBoundsParams p) {
+  const int token = blockIdx.x;
+  const int row = p.token_row[token];
+  if (row < 0 || row >= p.rows) {
+    if (threadIdx.x == 0) raise_status(kStatusBadRow);
+    return;
+  }
+  const int q0 = p.cu_seq_q[row], count = p.cu_seq_q[row + 1] - q0, end = p.seqused_k[row];
+  const int pos = end - count + (token - q0);
+  if (pos < 0 || pos >= end) return;
+  if (token != q0 && pos % kBlockKeys != 0) return;
+  const int first = pos - pos % kBlockKeys, n = min(kBlockKeys, end - first);
+  const int pidx = first / p.page_size;
+  const int page = pidx < p.width ? p.block_table[static_cast<int64_t>(row) * p.width + pidx] : -1;
+  if (page < 0 || page >= p.num_pages) {
+    if (threadIdx.x == 0) raise_status(kStatusBadPage);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int at = first % p.page_size;
+  for (int h = warp; h < p.kv_heads; h += kBoundsThreads / 32) {
+    const __nv_bfloat16* src =
+        p.keys + ((static_cast<int64_t>(page) * p.page_size + at) * p.kv_heads + h) * 128 + 4 * lane;
+    const int64_t step = static_cast<int64_t>(p.kv_heads) * 128;
+    __nv_bfloat162 lo[2], hi[2];
+    *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(src);
+    hi[0] = lo[0];
+    hi[1] = lo[1];
+#pragma unroll 16
+    for (int i = 1; i < kBlockKeys; ++i) {
+      if (i < n) {
+        __nv_bfloat162 v[2];
+        *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(src + i * step);
+        lo[0] = __hmin2_nan(lo[0], v[0]);
+        lo[1] = __hmin2_nan(lo[1], v[1]);
+        hi[0] = __hmax2_nan(hi[0], v[0]);
+        hi[1] = __hmax2_nan(hi[1], v[1]);
+      }
+    }
+    const int blocks = p.page_size / kBlockKeys;
+    __nv_bfloat16* dst =
+        p.bounds + ((static_cast<int64_t>(page) * p.kv_heads + h) * blocks + at / kBlockKeys) * 256 + 4 * lane;
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(lo);
+    *reinterpret_cast<uint2*>(dst + 128) = *reinterpret_cast<uint2*>(hi);
+  }
+}
+
+// ---------------------------------------------------------------- selection and attention
+struct SparseAttentionParams {
+  const __nv_bfloat16* q;       // [rows, H, 128]
+  __nv_bfloat16* out;           // [rows, H, 128]
+  const __nv_bfloat16* bounds;  // [num_pages, kv_heads, page_size / 64, 2, 128]
+  const int32_t* block_table;   // [rows, width]
+  const int32_t* seqused_k;     // [rows]
+  int32_t* selected;            // [rows, kv_heads, top] or null
+  int32_t width, num_pages, page_size, heads, kv_heads;
+  int32_t top, sink, recent;
+  float scale_log2;
+};
+
+constexpr int kSparseThreads = kDecSubThreads;
+constexpr int kSparseWarps = kSparseThreads / 32;
+// Keys, border indices and border scores of a row's blocks share the ring's memory.
+constexpr int kSparseMaxBlocks = kDecRingBytes / 16;
+constexpr int kSparseMaxTop = 1024;
+static_assert(kDecRingBytes % 16 == 0, "three arrays in the ring");
+
+// Order-preserving integers of scores: NaN above everything, -0 as +0.
+__device__ __forceinline__ uint32_t score_key(float s) {
+  if (s != s) return 0xFFFFFFFFu;
+  const uint32_t b = __float_as_uint(s + 0.f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long score_key(double s) {
+  if (s != s) return ~0ull;
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(s + 0.0));
+  return (b >> 63) ? ~b : (b | (1ull << 63));
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+__device__ __forceinline__ void cluster_store(uint32_t* local, uint32_t rank, uint32_t v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
+// The bounds of block b for KV head h, or null where the table names no page.
+__device__ __forceinline__ const __nv_bfloat16* block_bounds(const SparseAttentionParams& p, int row, int h, int b) {
+  const int per_page = p.page_size / kBlockKeys;
+  const int pidx = b / per_page;
+  const int page = p.block_table[static_cast<int64_t>(row) * p.width + pidx];
+  if (page < 0 || page >= p.num_pages) return nullptr;
+  return p.bounds + ((static_cast<int64_t>(page) * p.kv_heads + h) * per_page + b % per_page) * 256;
+}
+
+// Scores of blocks [b0, b1) (b0 a multiple of 8) into keys[], by the CTA's warps; returns the
+// lane's largest sum |terms|.
+template <int GROUP>
+__device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, int row, int h, int b0, int b1,
+                                              uint32_t* keys, int ranks) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, c4 = lane & 3;
+  // Query fragments: head g4, dims 32 j + 8 c4 .. + 7; the negative part, then the positive.
+  uint32_t qn[4][4], qp[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (g4 < GROUP)
+      v = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(row) * p.heads + h * GROUP + g4) * 128 + 32 * j +
+                                          8 * c4);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+      const __nv_bfloat162 n = __hmin2_nan(x, zero), m = __hmax2_nan(x, zero);
+      qn[j][i] = *reinterpret_cast<const uint32_t*>(&n);
+      qp[j][i] = *reinterpret_cast<const uint32_t*>(&m);
+    }
+  }
+  float worst = 0.f;
+  for (int base = b0 + 8 * warp; base < b1; base += 8 * kSparseWarps) {
+    const int b = base + g4;
+    const __nv_bfloat16* src = b < b1 ? block_bounds(p, row, h, b) : nullptr;
+    if (b < b1 && src == nullptr) raise_status(kStatusBadPage);
+    uint4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = src ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c4) : make_uint4(0, 0, 0, 0);
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr uint32_t kAbs = 0x7FFF7FFFu;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t* q = j < 4 ? qn[j & 3] : qp[j & 3];
+      const uint32_t f0[4] = {q[0], 0u, q[1], 0u}, f1[4] = {q[2], 0u, q[3], 0u};
+      mma_16816(s, f0, v[j].x, v[j].y);
+      mma_16816(s, f1, v[j].z, v[j].w);
+      const uint32_t e0[4] = {q[0] & kAbs, 0u, q[1] & kAbs, 0u}, e1[4] = {q[2] & kAbs, 0u, q[3] & kAbs, 0u};
+      mma_16816(a, e0, v[j].x & kAbs, v[j].y & kAbs);
+      mma_16816(a, e1, v[j].z & kAbs, v[j].w & kAbs);
+    }
+    // Head g4, blocks base + 2 c4 and + 1: the largest over the group's heads.
+    uint32_t k0 = g4 < GROUP ? score_key(s[0]) : 0u, k1 = g4 < GROUP ? score_key(s[1]) : 0u;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      k0 = max(k0, __shfl_xor_sync(0xffffffffu, k0, o));
+      k1 = max(k1, __shfl_xor_sync(0xffffffffu, k1, o));
+    }
+    const float big = fmaxf(a[0], a[1]);
+    worst = (a[0] < INFINITY && a[1] < INFINITY) ? fmaxf(worst, big) : INFINITY;
+    // Lane (g4, c4) hands the pair to CTA g4 (+ 8 for clusters beyond 8).
+    for (int r = g4; r < ranks; r += 8) {
+      if (base + 2 * c4 < b1) cluster_store(keys + base + 2 * c4, r, k0);
+      if (base + 2 * c4 + 1 < b1) cluster_store(keys + base + 2 * c4 + 1, r, k1);
+    }
+  }
+  return worst;
+}
+
+struct SparseShared {
+  uint64_t full[kDecStages], empty[kDecStages];
+  int abort_flag;
+  uint32_t worst;  // largest sum |terms| (float bits; the CTAs' maxima meet here)
+  int n_border, n_in, n_sel, digit, remaining;
+  uint32_t hist[256];
+  float merge_ml[kDecConsumerWarps][16][2];
+  float part[8][128];     // unnormalised output of each head of the group over this CTA's blocks
+  float part_ml[8][2];    // its running maximum and sum
+};
+
+// Exact score of block b (see the head of this file) by a whole warp, as an ordered integer.
+template <int GROUP>
+__device__ unsigned long long exact_score(const SparseAttentionParams& p, int row, int h, int b) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* src = block_bounds(p, row, h, b);
+  unsigned long long best = 0ull;
+  if (src == nullptr) return best;
+  const uint2 lo2 = *reinterpret_cast<const uint2*>(src + 4 * lane);
+  const uint2 hi2 = *reinterpret_cast<const uint2*>(src + 128 + 4 * lane);
+  const __nv_bfloat16 *lo = reinterpret_cast<const __nv_bfloat16*>(&lo2), *hi = reinterpret_cast<const __nv_bfloat16*>(&hi2);
+#pragma unroll 1
+  for (int g = 0; g < GROUP; ++g) {
+    const uint2 q2 = *reinterpret_cast<const uint2*>(p.q + (static_cast<int64_t>(row) * p.heads + h * GROUP + g) * 128 + 4 * lane);
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&q2);
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = __bfloat162float(q[i]);
+      const float n = x < 0.f ? x : (x == x ? 0.f : x), m = x > 0.f ? x : (x == x ? 0.f : x);
+      // A product of two bf16 values is exact in fp32's 24 bits (and in 64).
+      s += static_cast<double>(n) * static_cast<double>(__bfloat162float(lo[i]));
+      s += static_cast<double>(m) * static_cast<double>(__bfloat162float(hi[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    best = max(best, score_key(s));
+  }
+  return best;
+}
+
+// Turns keys[0 .. nb) into 1 (taken) or 0, with `need` of the blocks [sink, nb - recent) taken;
+// every thread of the CTA calls it. `index` and `score` are scratch for the blocks near the cut.
+template <int GROUP>
+__device__ void select_blocks(const SparseAttentionParams& p, int row, int h, int nb, int need, uint32_t* keys,
+                              uint32_t* index, unsigned long long* score, SparseShared& sh) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int c0 = p.sink, c1 = nb - p.recent;  // need <= c1 - c0, see the caller
+  uint32_t prefix = 0, known = 0;             // the cut's leading bits so far
+  int remaining = need;
+  if (need > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += kSparseThreads) sh.hist[i] = 0u;
+      __syncthreads();
+      for (int b = c0 + tid; b < c1; b += kSparseThreads)
+        if ((keys[b] & known) == prefix) atomicAdd(&sh.hist[(keys[b] >> shift) & 255u], 1u);
+      __syncthreads();
+      if (warp == 0) {  // bins from the top: lane l has 255 - 8 l .. 248 - 8 l
+        uint32_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += sh.hist[255 - 8 * lane - i];
+        uint32_t incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        uint32_t before = incl - sum;
+        if (before < static_cast<uint32_t>(remaining) && static_cast<uint32_t>(remaining) <= incl) {
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t n = sh.hist[255 - 8 * lane - i];
+            if (static_cast<uint32_t>(remaining) <= before + n) {
+              sh.digit = 255 - 8 * lane - i;
+              sh.remaining = remaining - static_cast<int>(before);
+              break;
+            }
+            before += n;
+          }
+        }
+      }
+      __syncthreads();
+      prefix |= static_cast<uint32_t>(sh.digit) << shift;
+      known |= 255u << shift;
+      remaining = sh.remaining;
+      __syncthreads();
+    }
+  }
+  // prefix is the need-th largest computed score.
+  const float eps2 = 2.f * 3.0517578125e-5f * __uint_as_float(sh.worst);  // 2 eps, eps = 2^-15 sum |terms|
+  const float cut = key_score(prefix);
+  uint32_t low = 0u, high = 0xFFFFFFFFu;  // every block between them (NaN included) is scored again
+  bool all = true;
+  if (eps2 < INFINITY && fabsf(cut) < INFINITY && prefix != 0xFFFFFFFFu) {
+    // One more step outwards for the rounding of these two sums.
+    low = score_key(__fsub_rd(cut, eps2));
+    high = score_key(__fadd_ru(cut, eps2));
+    all = false;
+  }
+  if (tid == 0) sh.n_border = sh.n_in = 0;
+  __syncthreads();
+  int in = 0;
+  for (int b = c0 + tid; b < c1; b += kSparseThreads) {
+    const uint32_t k = keys[b];
+    if (need <= 0 || (!all && k < low)) {
+      keys[b] = 0u;
+    } else if (!all && k > high) {
+      keys[b] = 1u;
+      ++in;
+    } else {
+      keys[b] = 0u;
+      index[atomicAdd(&sh.n_border, 1)] = static_cast<uint32_t>(b);
+    }
+  }
+  for (int b = tid; b < c0; b += kSparseThreads) keys[b] = 1u;
+  for (int b = c1 + tid; b < nb; b += kSparseThreads) keys[b] = 1u;
+  if (in) atomicAdd(&sh.n_in, in);
+  __syncthreads();
+  const int border = sh.n_border, left = need - sh.n_in;
+  if (left >= border) {  // all of them
+    for (int i = tid; i < border; i += kSparseThreads) keys[index[i]] = 1u;
+  } else if (left > 0) {
+    for (int i = warp; i < border; i += kSparseWarps) {
+      const unsigned long long s = exact_score<GROUP>(p, row, h, static_cast<int>(index[i]));
+      if (lane == 0) score[i] = s;
+    }
+    __syncthreads();
+    for (int i = tid; i < border; i += kSparseThreads) {
+      const unsigned long long s = score[i];
+      const uint32_t b = index[i];
+      int rank = 0;
+      for (int j = 0; j < border; ++j) rank += score[j] > s || (score[j] == s && index[j] < b);
+      if (rank < left) keys[b] = 1u;
+    }
+  }
+  __syncthreads();
+}
+
+// One cluster per (row, KV head): its CTAs score a share of the row's blocks each and hand the
+// scores to one another, select alike, attend to a share of the selected blocks each (the
+// decode ring and tile of attention_decode.cuh), and merge through shared memory. One launch,
+// no workspace.
+template <int GROUP>
+__global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(SparseAttentionParams p,
+                                                                            const __grid_constant__ CUtensorMap kmap,
+                                                                            const __grid_constant__ CUtensorMap vmap) {
+  extern __shared__ __align__(1024) uint8_t dsm[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
+  __shared__ SparseShared sh;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);
+  uint32_t* index = keys + kSparseMaxBlocks;
+  unsigned long long* score = reinterpret_cast<unsigned long long*>(index + kSparseMaxBlocks);
+  int* list = reinterpret_cast<int*>(smem + kDecRingBytes);  // [top] selected blocks, ascending
+  int* where = list + p.top;                                 // [top] first pool token, -1: no page
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+  const int h = blockIdx.y, row = blockIdx.z;
+  const int per_page = p.page_size / kBlockKeys;
+  int len = p.seqused_k[row];
+  if (len > p.width * p.page_size) {  // more keys than the table has pages for
+    if (tid == 0 && rank == 0) raise_status(kStatusBadPage);
+    len = p.width * p.page_size;
+  }
+  const int nb = len > 0 ? (len - 1) / kBlockKeys + 1 : 0;
+  if (tid == 0) {
+    for (int s = 0; s < kDecStages; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], kDecConsumerWarps);
+    }
+    sh.abort_flag = 0;
+    sh.worst = 0u;
+    fence_barrier_init();
+  }
+  const bool choose = nb > p.top;  // row-uniform: the whole cluster agrees
+  if (choose) {
+    if (ranks > 1) cluster_sync();  // every CTA of the cluster has started and set its words
+    else __syncthreads();
+    const int groups = (nb + 7) / 8;
+    const int b0 = 8 * (groups * rank / ranks), b1 = min(nb, 8 * (groups * (rank + 1) / ranks));
+    float worst = score_blocks<GROUP>(p, row, h, b0, b1, keys, ranks);
+    worst = warp_max(worst);
+    if (lane < ranks) {  // non-negative floats compare as their bits do
+      uint32_t a;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(&sh.worst)), "r"(lane));
+      asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(a), "r"(__float_as_uint(worst)) : "memory");
+    }
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+    select_blocks<GROUP>(p, row, h, nb, p.top - p.sink - p.recent, keys, index, score, sh);
+  }
+  if (warp == 0) {  // ascending list
+    int n = 0;
+    for (int b0 = 0; b0 < nb; b0 += 32) {
+      const int b = b0 + lane;
+      const bool take = b < nb && (!choose || keys[b] != 0u);
+      const unsigned m = __ballot_sync(0xffffffffu, take);
+      const int at = n + __popc(m & ((1u << lane) - 1u));
+      if (take && at < p.top) list[at] = b;
+      n += __popc(m);
+    }
+    if (lane == 0) sh.n_sel = min(n, p.top);  // min(nb, top)
+  }
+  __syncthreads();
+  const int n_sel = sh.n_sel;
+  for (int i = tid; i < n_sel; i += kSparseThreads) {
+    const int b = list[i];
+    const int page = p.block_table[static_cast<int64_t>(row) * p.width + b / per_page];
+    const bool ok = page >= 0 && page < p.num_pages;
+    if (!ok) raise_status(kStatusBadPage);
+    where[i] = ok ? page * p.page_size + (b % per_page) * kBlockKeys : -1;
+  }
+  if (p.selected != nullptr && rank == 0) {
+    int32_t* dst = p.selected + (static_cast<int64_t>(row) * p.kv_heads + h) * p.top;
+    for (int i = tid; i < p.top; i += kSparseThreads) dst[i] = i < n_sel ? list[i] : -1;
+  }
+  fence_proxy_async_smem();  // the ring's generic reads and writes precede its TMA fills
+  __syncthreads();
+
+  const int i0 = n_sel * rank / ranks, i1 = n_sel * (rank + 1) / ranks;  // this CTA's blocks
+  if (warp == kDecConsumerWarps) {
+    if (lane == 0) {
+      int t = 0;
+      for (int i = i0; i < i1; ++i) {
+        const int tok = where[i];
+        if (tok < 0) continue;
+        const int s = t % kDecStages;
+        if (t >= kDecStages && !mbar_wait(&sh.empty[s], ((t / kDecStages) - 1) & 1, &sh.abort_flag)) break;
+        uint8_t* stage = smem + s * kDecStageBytes;
+        mbar_expect_tx(&sh.full[s], kDecStageBytes);
+        tma_load_3d(stage, &kmap, &sh.full[s], 0, h, tok);
+        tma_load_3d(stage + kDecHalfBytes, &kmap, &sh.full[s], 64, h, tok);
+        tma_load_3d(stage + kDecTileBytes, &vmap, &sh.full[s], 0, h, tok);
+        tma_load_3d(stage + kDecTileBytes + kDecHalfBytes, &vmap, &sh.full[s], 64, h, tok);
+        ++t;
+      }
+      // Never leave with copies in flight.
+      if (sh.abort_flag)
+        for (int j = max(0, t - kDecStages); j < t; ++j) mbar_drain(&sh.full[j % kDecStages], (j / kDecStages) & 1);
+    }
+    __syncwarp();
+  } else {
+    AttentionParams ap{};
+    ap.q = p.q;
+    ap.heads = p.heads;
+    ap.scale_log2 = p.scale_log2;
+    DecodeUnit u{};
+    u.h = h;
+    u.row = row;
+    u.q0 = row;
+    u.count = 1;
+    u.end = u.ke = len;
+    u.qrows = GROUP;
+    u.key_split = kDecConsumerWarps;
+    u.kpw = kBlockKeys / kDecConsumerWarps;
+    u.mt = 0;
+    u.kpart = warp;
+    const int g4 = lane >> 2, c4 = lane & 3;
+    uint32_t qa[8][4];
+    decode_load_q<GROUP>(ap, u, lane, qa);
+    const int qpos_a = decode_qpos<GROUP>(u, g4), qpos_b = -1;
+    float acc[16][4];
+#pragma unroll
+    for (int n = 0; n < 16; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+    int t = 0;
+    for (int i = i0; i < i1; ++i) {
+      if (where[i] < 0) continue;
+      const int s = t % kDecStages;
+      if (!mbar_wait(&sh.full[s], (t / kDecStages) & 1, &sh.abort_flag)) break;
+      decode_tile<GROUP>(ap, u, smem + s * kDecStageBytes, list[i] * kBlockKeys, lane, qpos_a, qpos_b, qa, acc, m_a, m_b,
+                         l_a, l_b);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[s]);
+      ++t;
+    }
+    l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
+    l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
+    l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
+    l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
+    named_barrier_sync(1, kDecConsumerWarps * 32);  // the ring is idle: it becomes the merge scratch
+    // After a wait that gave up this merges garbage, but every warp still meets every barrier.
+    decode_merge(u, warp, lane, reinterpret_cast<float*>(smem), sh.merge_ml, acc, m_a, m_b, l_a, l_b,
+                 [] { named_barrier_sync(1, kDecConsumerWarps * 32); });
+    if (warp == 0 && g4 < GROUP) {
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        sh.part[g4][n * 8 + 2 * c4] = acc[n][0];
+        sh.part[g4][n * 8 + 2 * c4 + 1] = acc[n][1];
+      }
+      if (c4 == 0) {
+        sh.part_ml[g4][0] = m_a;
+        sh.part_ml[g4][1] = l_a;
+      }
+    }
+    __syncwarp();
+  }
+  if (ranks > 1) cluster_sync();
+  else __syncthreads();
+  // out = sum_c 2^(m_c - m) acc_c / sum_c 2^(m_c - m) l_c, in rank order; a row without keys gives 0
+  // (den is 0 then alone: a NaN or infinite score leaves den NaN, and shows).
+  for (int i = rank * kSparseThreads + tid; i < GROUP * 128; i += ranks * kSparseThreads) {
+    const int g = i / 128, d = i % 128;
+    float mx = -INFINITY, num = 0.f, den = 0.f;
+    for (int r = 0; r < ranks; ++r) mx = fmaxf(mx, cluster_load(&sh.part_ml[g][0], r));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    for (int r = 0; r < ranks; ++r) {
+      const float w = exp2f(cluster_load(&sh.part_ml[g][0], r) - base);
+      num += w * cluster_load(&sh.part[g][d], r);
+      den += w * cluster_load(&sh.part_ml[g][1], r);
+    }
+    p.out[(static_cast<int64_t>(row) * p.heads + h * GROUP + g) * 128 + d] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+  }
+  if (ranks > 1) cluster_sync();  // the parts stay until every CTA has read them
+}
+
+}  // namespace hb

@@ -15,9 +15,12 @@
 #include "../../include/helios_b200.h"
 #include "attention_decode.cuh"
 #include "attention_prefill.cuh"
+#include "attention_sparse.cuh"
 #include "gemm_swiglu.cuh"
 #include "hb_common.cuh"
+#include "linear_w4.cuh"
 #include "lm_head_argmax.cuh"
+#include "logit_controls.cuh"
 #include "model_ops.cuh"
 #include "norm_rope_append.cuh"
 #include "prefix_index.cuh"
@@ -121,6 +124,7 @@ int ensure_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 bool g_dec_smem[4][64], g_decp_smem[4][64], g_pre_smem[4][64], g_prx_smem[4][64], g_tick_smem[64], g_gemm_smem[64], g_argmax_smem[64];
+bool g_sparse_smem[4][64], g_control_smem[64];
 
 constexpr int kDefaultOverlapDecodeSms = 100;
 
@@ -155,6 +159,24 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t 
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Launch with thread-block clusters of `cluster` CTAs along x.
+template <typename... Params, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(Params...), dim3 grid, dim3 block, unsigned cluster, size_t smem,
+                           cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
@@ -740,6 +762,159 @@ int hb_lm_head_argmax(const void* x, int32_t m, int32_t k, const void* weight, i
     return rc;
   hb::argmax_finalize_kernel<<<(m + 127) / 128, 128, 0, stream>>>(best, m, out_ids);
   return check_launch("argmax_finalize_kernel");
+}
+
+int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const int32_t* packed, const void* scales,
+                 const uint8_t* zeros, int32_t n, int32_t group, void* out, cudaStream_t stream) {
+  if (m < 0 || k < 1 || n < 1 || x_stride < k) return fail(HB_ERR_INVALID, "bad 4-bit projection sizes");
+  if (group != 32 && group != 64 && group != 128)
+    return fail(HB_ERR_UNSUPPORTED, "4-bit weights come in groups of 32, 64 or 128 (got %d)", group);
+  if (k % group != 0) return fail(HB_ERR_INVALID, "k (%d) must be a multiple of the group size %d", k, group);
+  if (n > 65535 * hb::kW4Rows) return fail(HB_ERR_UNSUPPORTED, "4-bit projection: n %d is too large", n);
+  if (m == 0) return HB_OK;
+  if (x == nullptr || packed == nullptr || scales == nullptr || out == nullptr || !aligned(x, 16) ||
+      !aligned(packed, 16) || !aligned(scales, 2) || !aligned(out, 2) || x_stride % 8 != 0)
+    return fail(HB_ERR_INVALID, "4-bit projection pointers must be non-null, x rows and packed 16-byte aligned");
+  hb::LinearW4Params p{static_cast<const __nv_bfloat16*>(x), x_stride, reinterpret_cast<const uint32_t*>(packed),
+                       static_cast<const __nv_bfloat16*>(scales), zeros, static_cast<__nv_bfloat16*>(out), m, n, k};
+  const int tiles = (n + hb::kW4Rows - 1) / hb::kW4Rows;
+  const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
+  const int token_tiles = (m + 8 * nt - 1) / (8 * nt);
+  if (token_tiles > 65535) return fail(HB_ERR_UNSUPPORTED, "4-bit projection: too many token rows (%d)", m);
+  int splits = 1;
+  while (splits < 4 && static_cast<int64_t>(tiles) * token_tiles * splits < 2 * 148 && k / (splits * 2) >= 1024) splits *= 2;
+  cudaError_t e = cudaSuccess;
+#define HB_W4_LAUNCH(G, NT)                                                                                \
+  e = launch_cluster(hb::linear_w4_kernel<G, NT>, dim3(splits, tiles, token_tiles), dim3(32 * hb::kW4Warps), \
+                     splits, 0, stream, p)
+#define HB_W4_GROUP(G)                  \
+  do {                                  \
+    if (nt == 1) HB_W4_LAUNCH(G, 1);    \
+    else if (nt == 2) HB_W4_LAUNCH(G, 2); \
+    else HB_W4_LAUNCH(G, 4);            \
+  } while (0)
+  if (group == 128) HB_W4_GROUP(128);
+  else if (group == 64) HB_W4_GROUP(64);
+  else HB_W4_GROUP(32);
+#undef HB_W4_GROUP
+#undef HB_W4_LAUNCH
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "linear_w4_kernel: %s", cudaGetErrorString(e));
+  return check_launch("linear_w4_kernel");
+}
+
+int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_pages, int32_t page_size,
+                        const int32_t* block_table, int32_t width, const int32_t* cu_seq_q, const int32_t* seqused_k,
+                        const int32_t* token_row, int32_t num_rows, int32_t total_tokens, int32_t kv_heads,
+                        int32_t head_dim, cudaStream_t stream) {
+  if (head_dim != 128) return fail(HB_ERR_UNSUPPORTED, "key block bounds support head_dim 128, got %d", head_dim);
+  if (page_size < hb::kBlockKeys || page_size % hb::kBlockKeys != 0)
+    return fail(HB_ERR_INVALID, "page_size must be a multiple of %d", hb::kBlockKeys);
+  if (num_pages < 1 || width < 1 || num_rows < 0 || total_tokens < 0 || kv_heads < 1)
+    return fail(HB_ERR_INVALID, "bad key block sizes");
+  if (num_pages * page_size > (int64_t(1) << 31)) return fail(HB_ERR_UNSUPPORTED, "pool exceeds 2^31 tokens");
+  if (total_tokens == 0 || num_rows == 0) return HB_OK;
+  if (key_pool == nullptr || bounds == nullptr || block_table == nullptr || cu_seq_q == nullptr ||
+      seqused_k == nullptr || token_row == nullptr || !aligned(key_pool, 16) || !aligned(bounds, 16))
+    return fail(HB_ERR_INVALID, "key block pointers must be non-null, pool and bounds 16-byte aligned");
+  hb::BlockBoundsParams p{static_cast<const __nv_bfloat16*>(key_pool), static_cast<__nv_bfloat16*>(bounds), block_table,
+                          cu_seq_q, seqused_k, token_row, num_rows, total_tokens, width,
+                          static_cast<int32_t>(num_pages), page_size, kv_heads};
+  hb::key_block_bounds_kernel<<<total_tokens, hb::kBoundsThreads, 0, stream>>>(p);
+  return check_launch("key_block_bounds_kernel");
+}
+
+int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* value_pool, const void* bounds,
+                              int64_t num_pages, int32_t page_size, const int32_t* block_table, int32_t width,
+                              const int32_t* seqused_k, int32_t num_rows, int32_t heads, int32_t kv_heads,
+                              int32_t head_dim, int32_t top_blocks, int32_t sink_blocks, int32_t recent_blocks,
+                              float scale, int32_t* selected, void* out, cudaStream_t stream) {
+  if (head_dim != 128) return fail(HB_ERR_UNSUPPORTED, "sparse attention supports head_dim 128, got %d", head_dim);
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads) return fail(HB_ERR_INVALID, "bad head counts");
+  const int group = heads / kv_heads;
+  if (group != 1 && group != 2 && group != 4 && group != 8)
+    return fail(HB_ERR_UNSUPPORTED, "query heads per KV head must be 1, 2, 4 or 8 (got %d)", group);
+  if (page_size < hb::kBlockKeys || page_size % hb::kBlockKeys != 0)
+    return fail(HB_ERR_INVALID, "page_size must be a multiple of %d", hb::kBlockKeys);
+  if (num_pages < 1 || width < 1 || num_rows < 0 || num_rows > 65535 || kv_heads > 65535)
+    return fail(HB_ERR_INVALID, "bad sparse attention sizes");
+  if (num_pages * page_size > (int64_t(1) << 31)) return fail(HB_ERR_UNSUPPORTED, "pool exceeds 2^31 tokens");
+  if (static_cast<int64_t>(width) * (page_size / hb::kBlockKeys) > hb::kSparseMaxBlocks)
+    return fail(HB_ERR_UNSUPPORTED, "sparse attention covers %d tokens per row at most", hb::kSparseMaxBlocks * hb::kBlockKeys);
+  if (sink_blocks < 0 || recent_blocks < 1 || top_blocks > hb::kSparseMaxTop || sink_blocks > top_blocks ||
+      recent_blocks > top_blocks - sink_blocks)
+    return fail(HB_ERR_INVALID, "top_blocks must hold sink_blocks >= 0 and recent_blocks >= 1, and be at most %d",
+                hb::kSparseMaxTop);
+  if (num_rows == 0) return HB_OK;
+  if (q == nullptr || key_pool == nullptr || value_pool == nullptr || bounds == nullptr || block_table == nullptr ||
+      seqused_k == nullptr || out == nullptr || !aligned(q, 16) || !aligned(key_pool, 16) || !aligned(value_pool, 16) ||
+      !aligned(bounds, 16) || !aligned(out, 16))
+    return fail(HB_ERR_INVALID, "sparse attention pointers must be non-null and 16-byte aligned");
+  CUtensorMap kmap, vmap;
+  const uint64_t pool_tokens = static_cast<uint64_t>(num_pages) * page_size;
+  const uint64_t row_bytes = static_cast<uint64_t>(kv_heads) * head_dim * 2;
+  if (int rc = encode_3d(&kmap, key_pool, head_dim, kv_heads, pool_tokens, head_dim * 2, row_bytes, 64, 1, hb::kBlockKeys))
+    return rc;
+  if (int rc = encode_3d(&vmap, value_pool, head_dim, kv_heads, pool_tokens, head_dim * 2, row_bytes, 64, 1, hb::kBlockKeys))
+    return rc;
+  hb::SparseAttentionParams p{static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out),
+                              static_cast<const __nv_bfloat16*>(bounds), block_table, seqused_k, selected, width,
+                              static_cast<int32_t>(num_pages), page_size, heads, kv_heads, top_blocks, sink_blocks,
+                              recent_blocks, scale * 1.4426950408889634f};
+  const int gs = group_slot(group);
+  const size_t smem = hb::kDecSmemBytes + 8 * static_cast<size_t>(top_blocks);
+  const int most = hb::kDecSmemBytes + 8 * hb::kSparseMaxTop;
+  int ranks = 1;
+  while (ranks < 8 && 2 * ranks <= top_blocks && static_cast<int64_t>(num_rows) * kv_heads * ranks * 2 <= 2 * 148) ranks *= 2;
+  const dim3 grid(ranks, kv_heads, num_rows);
+  cudaError_t e = cudaSuccess;
+#define HB_SPARSE(G)                                                                                          \
+  do {                                                                                                        \
+    if (int rc = ensure_smem(hb::sparse_attention_kernel<G>, most, g_sparse_smem[gs])) return rc;             \
+    e = launch_cluster(hb::sparse_attention_kernel<G>, grid, dim3(hb::kSparseThreads), ranks, smem, stream, p, kmap, \
+                       vmap);                                                                                 \
+  } while (0)
+  switch (group) {
+    case 1: HB_SPARSE(1); break;
+    case 2: HB_SPARSE(2); break;
+    case 4: HB_SPARSE(4); break;
+    default: HB_SPARSE(8); break;
+  }
+#undef HB_SPARSE
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "sparse_attention_kernel: %s", cudaGetErrorString(e));
+  return check_launch("sparse_attention_kernel");
+}
+
+int hb_control_logits(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab, const float* repetition,
+                      const float* frequency, const float* presence, const int32_t* history, int32_t history_rows,
+                      int64_t history_width, const int32_t* slots, const int32_t* lengths,
+                      const int32_t* prompt_lengths, const int32_t* bias_offsets, const int32_t* bias_tokens,
+                      const float* bias_values, int32_t bias_entries, const int32_t* mask, int32_t masks,
+                      const int32_t* mask_rows, void* out, int64_t out_stride, cudaStream_t stream) {
+  if (rows < 0 || rows > 65535 || vocab < 1 || row_stride < vocab || out_stride < vocab)
+    return fail(HB_ERR_INVALID, "bad logit control sizes");
+  if (rows == 0) return HB_OK;
+  if (logits == nullptr || out == nullptr) return fail(HB_ERR_INVALID, "null logits");
+  if (logits == out && row_stride != out_stride) return fail(HB_ERR_INVALID, "in place needs equal row strides");
+  if (history != nullptr && (slots == nullptr || lengths == nullptr || prompt_lengths == nullptr || history_rows < 1 ||
+                             history_width < 1 || history_width > INT32_MAX))
+    return fail(HB_ERR_INVALID, "a history needs its slots, lengths and prompt lengths");
+  if (bias_offsets != nullptr && (bias_entries < 0 || (bias_entries > 0 && (bias_tokens == nullptr || bias_values == nullptr))))
+    return fail(HB_ERR_INVALID, "bias offsets need tokens and values");
+  if (mask != nullptr && (mask_rows == nullptr || masks < 1)) return fail(HB_ERR_INVALID, "a mask needs its row numbers");
+  unsigned ranks = 8;
+  while (ranks > 1 && vocab <= 1024 * static_cast<int>(ranks)) ranks /= 2;
+  int segment = (vocab + static_cast<int>(ranks) - 1) / static_cast<int>(ranks);
+  segment = std::min((segment + 31) / 32 * 32, hb::kControlMaxSegment);
+  hb::LogitControlParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<__nv_bfloat16*>(out), row_stride,
+                           out_stride, rows, vocab, repetition, frequency, presence, history, history_width,
+                           history_rows, slots, lengths, prompt_lengths, bias_offsets, bias_tokens, bias_values, bias_entries,
+                           reinterpret_cast<const uint32_t*>(mask), masks, (vocab + 31) / 32, mask_rows, segment};
+  constexpr int most = hb::kControlMaxSegment * 4 + hb::kControlMaxSegment / 8;
+  if (int rc = ensure_smem(hb::logit_controls_kernel, most, g_control_smem)) return rc;
+  const cudaError_t e = launch_cluster(hb::logit_controls_kernel, dim3(ranks, rows), dim3(hb::kControlThreads), ranks,
+                                       static_cast<size_t>(segment) * 4 + segment / 8, stream, p);
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "logit_controls_kernel: %s", cudaGetErrorString(e));
+  return check_launch("logit_controls_kernel");
 }
 
 int hb_hash_token_blocks(const int32_t* tokens, const int64_t* offsets, int32_t prompts, int32_t block_size,

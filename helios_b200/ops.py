@@ -207,6 +207,209 @@ def lm_head_argmax(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | No
     return out
 
 
+def _together(device: torch.device, **tensors: torch.Tensor | None) -> None:
+    """Every given tensor on ``device``, contiguous."""
+    for name, t in tensors.items():
+        if t is not None:
+            if t.device != device:
+                raise ValueError(f"{name} must be on {device}, got {t.device}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """Run an entry point on ``device``'s current stream, with that device current."""
+    fn = getattr(lib(), name)
+    stream = _stream(device)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc:
+        _native.check(rc, name)
+
+
+def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x [m, k] @ W^T`` (bf16 ``[m, n]``) for a weight held in 4 bits: ``W[j, i] = (q[j, i] -
+    z[g, j]) * scales[g, j]``, ``g = i // group``. ``packed`` int32 ``[n, k / 8]`` (word c: even i's
+    in the low half, odd i's in the high half, see hb_linear_w4), ``scales`` bf16 ``[k / group, n]``,
+    ``zeros`` uint8 ``[k / group, n]`` (None: 8); groups of 32, 64 or 128. ``x`` may have any row
+    stride that keeps its rows 16-byte aligned. ``helios_b200.w4.quantize_w4`` makes the three
+    tensors from a weight. Returns ``out``, or a new tensor."""
+    _need(x, BF16, "x", contiguous=False)
+    _need(packed, torch.int32, "packed")
+    _need(scales, BF16, "scales")
+    if x.dim() != 2 or packed.dim() != 2 or scales.dim() != 2:
+        raise ValueError("x, packed and scales must be 2-D")
+    m, k = x.shape
+    n, groups = packed.shape[0], scales.shape[0]
+    if packed.shape[1] * 8 != k or scales.shape[1] != n or groups == 0 or k % groups:
+        raise ValueError("packed must be [n, k / 8] and scales [k / group, n] for x [m, k]")
+    if x.stride(1) != 1:
+        raise ValueError("x rows must be contiguous")
+    if zeros is not None:
+        _need(zeros, torch.uint8, "zeros")
+        if zeros.shape != scales.shape:
+            raise ValueError("zeros must have the shape of scales")
+    dev = x.device
+    if out is None:
+        out = torch.empty((m, n), dtype=BF16, device=dev)
+    else:
+        _need(out, BF16, "out")
+        if out.shape != (m, n):
+            raise ValueError("out must be [m, n]")
+    _together(dev, packed=packed, scales=scales, zeros=zeros, out=out)
+    _call("hb_linear_w4", dev, x.data_ptr(), x.stride(0) if m > 1 else k, m, k, packed.data_ptr(), scales.data_ptr(),
+          _ptr(zeros), n, k // groups, out.data_ptr())
+    return out
+
+
+BLOCK_KEYS = 64  # keys per block of the sparse attention
+
+
+def _check_bounds(key_pool: torch.Tensor, bounds: torch.Tensor) -> None:
+    _need(key_pool, BF16, "key_pool")
+    _need(bounds, BF16, "bounds")
+    pages, page, heads, dim = key_pool.shape
+    if bounds.shape != (pages, heads, page // BLOCK_KEYS, 2, dim):
+        raise ValueError("bounds must be [pages, kv_heads, page / 64, 2, head_dim] for the key pool")
+
+
+def key_block_bounds(key_pool: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor,
+                     cu_seq_q: torch.Tensor, seqused_k: torch.Tensor, token_row: torch.Tensor) -> torch.Tensor:
+    """Bring ``bounds`` up to date with the keys a tick appended (hb_key_block_bounds): one layer's
+    ``key_pool [pages, page, Hkv, d]`` and ``bounds [pages, Hkv, page / 64, 2, d]``, with the tick's
+    ``block_table [rows, width]``, ``cu_seq_q [rows + 1]``, ``seqused_k [rows]`` and ``token_row
+    [tokens]`` (all int32). Only blocks holding new positions are written. Returns ``bounds``."""
+    _check_bounds(key_pool, bounds)
+    for name, t in (("block_table", block_table), ("cu_seq_q", cu_seq_q), ("seqused_k", seqused_k),
+                    ("token_row", token_row)):
+        _need(t, torch.int32, name)
+    rows, width = block_table.shape
+    if cu_seq_q.numel() != rows + 1 or seqused_k.numel() != rows:
+        raise ValueError("cu_seq_q needs rows + 1 entries and seqused_k rows")
+    dev = key_pool.device
+    _together(dev, bounds=bounds, block_table=block_table, cu_seq_q=cu_seq_q, seqused_k=seqused_k,
+              token_row=token_row)
+    _call("hb_key_block_bounds", dev, key_pool.data_ptr(), bounds.data_ptr(), key_pool.shape[0], key_pool.shape[1],
+          block_table.data_ptr(), width, cu_seq_q.data_ptr(), seqused_k.data_ptr(), token_row.data_ptr(), rows,
+          token_row.numel(), key_pool.shape[2], key_pool.shape[3])
+    return bounds
+
+
+def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, bounds: torch.Tensor,
+                           block_table: torch.Tensor, seqused_k: torch.Tensor, out: torch.Tensor | None = None, *,
+                           top_blocks: int, sink_blocks: int = 1, recent_blocks: int = 2,
+                           scale: float | None = None, selected: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one query token per row, ``q [rows, H, d]``, over the ``top_blocks`` 64-key blocks
+    that the ``bounds`` of key_block_bounds select for it and each KV head, the row's first
+    ``sink_blocks`` and last ``recent_blocks`` always among them (hb_sparse_paged_attention).
+    ``selected`` (int32 ``[rows, Hkv, top_blocks]``) gets the blocks in ascending order, then -1.
+    Returns ``out [rows, H, d]``, or a new tensor; a row without keys gives zeros."""
+    _need(q, BF16, "q")
+    _need(value_pool, BF16, "value_pool")
+    _check_bounds(key_pool, bounds)
+    _need(block_table, torch.int32, "block_table")
+    _need(seqused_k, torch.int32, "seqused_k")
+    rows, heads, dim = q.shape
+    pages, page, kv_heads, pool_dim = key_pool.shape
+    if value_pool.shape != key_pool.shape or dim != pool_dim:
+        raise ValueError("key and value pools must match each other and the query's head_dim")
+    if block_table.dim() != 2 or block_table.shape[0] != rows or seqused_k.numel() != rows:
+        raise ValueError("block_table and seqused_k need one row per query row")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need(out, BF16, "out")
+        if out.shape != q.shape:
+            raise ValueError("out must have the shape of q")
+    if selected is not None:
+        _need(selected, torch.int32, "selected")
+        if selected.shape != (rows, kv_heads, top_blocks):
+            raise ValueError("selected must be [rows, kv_heads, top_blocks]")
+    dev = q.device
+    _together(dev, key_pool=key_pool, value_pool=value_pool, bounds=bounds, block_table=block_table,
+              seqused_k=seqused_k, out=out, selected=selected)
+    _call("hb_sparse_paged_attention", dev, q.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
+          bounds.data_ptr(), pages, page, block_table.data_ptr(), block_table.shape[1], seqused_k.data_ptr(), rows,
+          heads, kv_heads, dim, top_blocks, sink_blocks, recent_blocks, dim ** -0.5 if scale is None else float(scale),
+          _ptr(selected), out.data_ptr())
+    return out
+
+
+def control_logits(logits: torch.Tensor, *, repetition: torch.Tensor | None = None,
+                   frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                   history: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+                   lengths: torch.Tensor | None = None, prompt_lengths: torch.Tensor | None = None,
+                   bias: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+                   mask: torch.Tensor | None = None, mask_rows: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties, biases and grammar masks on ``logits [rows, V]`` (bf16, rows may be strided), as
+    hb_control_logits defines them. ``repetition`` / ``frequency`` / ``presence``: fp32 ``[rows]``
+    (None: 1, 0, 0), applied to the tokens of ``history`` (int32 ``[slots, width]``; row r's is
+    ``history[slots[r], :lengths[slots[r]]]``, its first ``prompt_lengths[slots[r]]`` the prompt;
+    slot -1: none). ``bias``: int32 offsets ``[rows + 1]``, int32 tokens (ascending within a row) and
+    fp32 values. ``mask`` int32 ``[masks, ceil(V / 32)]`` with ``mask_rows`` int32 ``[rows]`` (-1: none).
+    Returns ``out`` (``logits`` itself works in place), or a new tensor."""
+    _need(logits, BF16, "logits", contiguous=False)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be [rows, V] with contiguous rows")
+    rows, vocab = logits.shape
+    dev = logits.device
+    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        if t is not None:
+            _need(t, torch.float32, name)
+            if t.numel() != rows:
+                raise ValueError(f"{name} needs one value per row")
+    history_rows = history_width = 0
+    if history is not None:
+        if slots is None or lengths is None or prompt_lengths is None:
+            raise ValueError("a history needs slots, lengths and prompt_lengths")
+        for name, t in (("history", history), ("slots", slots), ("lengths", lengths),
+                        ("prompt_lengths", prompt_lengths)):
+            _need(t, torch.int32, name)
+        if history.dim() != 2:
+            raise ValueError("history must be [slots, width]")
+        history_rows, history_width = history.shape
+        if slots.numel() != rows or lengths.numel() != history_rows or prompt_lengths.numel() != history_rows:
+            raise ValueError("slots needs one entry per row, lengths and prompt_lengths one per history row")
+    offsets = tokens = values = None
+    if bias is not None:
+        offsets, tokens, values = bias
+        _need(offsets, torch.int32, "bias offsets")
+        _need(tokens, torch.int32, "bias tokens")
+        _need(values, torch.float32, "bias values")
+        if offsets.numel() != rows + 1 or tokens.numel() != values.numel():
+            raise ValueError("bias needs rows + 1 offsets and as many values as tokens")
+    masks = 0
+    if mask is not None:
+        _need(mask, torch.int32, "mask")
+        if mask_rows is None:
+            raise ValueError("a mask needs mask_rows")
+        _need(mask_rows, torch.int32, "mask_rows")
+        masks = mask.shape[0]
+        if mask.dim() != 2 or mask.shape[1] != (vocab + 31) // 32 or mask_rows.numel() != rows:
+            raise ValueError("mask must be [masks, ceil(V / 32)] and mask_rows [rows]")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=BF16, device=dev)
+    elif out is not logits:
+        _need(out, BF16, "out")
+        if out.shape != logits.shape or out.device != dev:
+            raise ValueError("out must have the shape and device of logits")
+    _together(dev, repetition=repetition, frequency=frequency, presence=presence, history=history, slots=slots,
+              lengths=lengths, prompt_lengths=prompt_lengths, bias_offsets=offsets, bias_tokens=tokens,
+              bias_values=values, mask=mask, mask_rows=mask_rows)
+    wide = rows > 1
+    _call("hb_control_logits", dev, logits.data_ptr(), logits.stride(0) if wide else vocab, rows, vocab,
+          _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(history), history_rows, history_width, _ptr(slots),
+          _ptr(lengths), _ptr(prompt_lengths), _ptr(offsets), _ptr(tokens), _ptr(values),
+          0 if tokens is None else tokens.numel(), _ptr(mask), masks,
+          _ptr(mask_rows), out.data_ptr(), out.stride(0) if wide else vocab)
+    return out
+
+
 def embedding(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     if ids.dtype != torch.long or not ids.is_cuda or not ids.is_contiguous():
         raise ValueError("token ids must be a contiguous CUDA int64 tensor")

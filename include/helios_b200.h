@@ -244,6 +244,76 @@ HB_API int hb_lm_head_argmax(const void* x, int32_t m, int32_t k, const void* we
                              unsigned long long* best, int64_t* out_ids, cudaStream_t stream);
 
 /*
+ * Projection with 4-bit weights (no counterpart in the reference, whose projections are bf16
+ * nn.Linear, src/helios/runtime/qwen3/layers.py:26-27,131-146).
+ *   out[t][j] = bf16(sum_g scales[g][j] * sum_{i in group g} (q[j][i] - z[g][j]) * x[t][i])
+ * x bf16 [m] rows of k elements, x_stride elements apart (16-byte aligned rows); packed int32
+ * [n][k / 8]: word c of a row holds i = 8c .. 8c + 7, the even i in its low 16 bits and the odd
+ * i in its high 16 bits, four bits each in ascending i; scales bf16 [k / group][n]; zeros uint8
+ * [k / group][n] with values 0 .. 15 (the low four bits are used), null for 8 everywhere; group
+ * 32, 64 or 128, k a multiple of it; out bf16 [m][n].
+ */
+HB_API int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const int32_t* packed,
+                        const void* scales, const uint8_t* zeros, int32_t n, int32_t group, void* out,
+                        cudaStream_t stream);
+
+/*
+ * Bounds of the 64-key blocks that a tick wrote (no counterpart in the reference). For every
+ * block of a row that holds one of the row's new positions (the last cu_seq_q[r+1] - cu_seq_q[r]
+ * of its seqused_k[r]), the elementwise minimum and maximum of the row's keys in it (NaN where a
+ * key is NaN) go to bounds bf16 [num_pages][kv_heads][page_size / 64][2][head_dim] (minimum,
+ * then maximum). One layer's key pool [num_pages][page_size][kv_heads][head_dim], head_dim 128;
+ * block_table, cu_seq_q, seqused_k and token_row (int32 [total_tokens]) as hb_tick_pack writes
+ * them. Other blocks' bounds stay.
+ */
+HB_API int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_pages, int32_t page_size,
+                               const int32_t* block_table, int32_t width, const int32_t* cu_seq_q,
+                               const int32_t* seqused_k, const int32_t* token_row, int32_t num_rows,
+                               int32_t total_tokens, int32_t kv_heads, int32_t head_dim, cudaStream_t stream);
+
+/*
+ * Sparse decode attention (no counterpart in the reference): one query token per row, attending
+ * to the 64-key blocks that the bounds select. Row r has seqused_k[r] keys (0 or less: zeros are
+ * written). A row of at most top_blocks blocks attends to all of them. Otherwise each KV head
+ * takes the row's first sink_blocks and last recent_blocks blocks and, of the others, those with
+ * the largest max over the head's query group of sum_d max(q_d lo_d, q_d hi_d), top_blocks in
+ * all; equal scores go to the lower block, NaN ranks first. Scores are compared exactly.
+ * q and out bf16 [num_rows][heads][head_dim]; selected int32 [num_rows][kv_heads][top_blocks]
+ * (may be null) gets the blocks in ascending order, then -1. Needs head_dim 128, 1, 2, 4 or 8
+ * query heads per KV head, top_blocks <= 1024 and width * page_size <= 393,216 tokens.
+ */
+HB_API int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* value_pool, const void* bounds,
+                                     int64_t num_pages, int32_t page_size, const int32_t* block_table, int32_t width,
+                                     const int32_t* seqused_k, int32_t num_rows, int32_t heads, int32_t kv_heads,
+                                     int32_t head_dim, int32_t top_blocks, int32_t sink_blocks,
+                                     int32_t recent_blocks, float scale, int32_t* selected, void* out,
+                                     cudaStream_t stream);
+
+/*
+ * Request controls on logits ahead of hb_sample (no counterpart in the reference, whose sampler
+ * knows temperature and top-p only, src/helios/runtime/qwen3/decode.py:457-473). Per row, in
+ * fp32 and in this order: a token of the row's history takes the repetition penalty (x > 0 ?
+ * x / r : x * r); one that occurs c > 0 times past the prompt loses frequency * c, then
+ * presence; a listed token gains its bias; a token the row's mask does not allow becomes -inf.
+ * The result is rounded once to bf16. Each control may be null.
+ *   history         int32 [history_rows][history_width]; row r uses row slots[r] (-1: none), its
+ *                   first lengths[slot] entries, of which the first prompt_lengths[slot] are prompt
+ *   bias_offsets    int32 [rows + 1] into bias_tokens / bias_values [bias_entries]; tokens ascend within a row,
+ *                   of equal neighbours the last counts, a token followed by a smaller one is
+ *                   skipped and flagged (HB_STATUS_BAD_TOKEN)
+ *   mask            int32 [masks][ceil(vocab / 32)], bit i of word c allows token 32c + i; row r
+ *                   uses mask mask_rows[r] (-1: none). A mask without a token leaves a row of -inf.
+ * out bf16 rows out_stride apart, or logits itself (then only changed values are written).
+ */
+HB_API int hb_control_logits(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab,
+                             const float* repetition, const float* frequency, const float* presence,
+                             const int32_t* history, int32_t history_rows, int64_t history_width,
+                             const int32_t* slots, const int32_t* lengths, const int32_t* prompt_lengths,
+                             const int32_t* bias_offsets, const int32_t* bias_tokens, const float* bias_values,
+                             int32_t bias_entries, const int32_t* mask, int32_t masks, const int32_t* mask_rows,
+                             void* out, int64_t out_stride, cudaStream_t stream);
+
+/*
  * Prefix-cache block keys (replaces hash_token_blocks / build_token_blocks,
  * src/helios/runtime/prefix_cache.py:86-110, as PrefixCache.longest_prefix and
  * store_completed_blocks call them, :208-260). Prompt p is tokens[offsets[p], offsets[p+1])
