@@ -17,6 +17,7 @@
 #include "attention_prefill.cuh"
 #include "attention_sparse.cuh"
 #include "gemm_swiglu.cuh"
+#include "gemm_w4.cuh"
 #include "hb_common.cuh"
 #include "linear_w4.cuh"
 #include "lm_head_argmax.cuh"
@@ -99,6 +100,21 @@ int encode_2d(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, 
   return HB_OK;
 }
 
+// 2-D map over packed 4-bit weights, int32 [rows][words]: box (32 words, 128 rows), 128-byte swizzle.
+int encode_packed(CUtensorMap* map, const void* base, uint64_t words, uint64_t rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(HB_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {words, rows};
+  const cuuint64_t strides[1] = {words * 4};
+  const cuuint32_t box[2] = {hb::kW4gPackedK / 8, hb::kW4gRows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HB_ERR_CUDA, "cuTensorMapEncodeTiled (packed) failed (%d)", static_cast<int>(r));
+  return HB_OK;
+}
+
 int sm_count() {
   static int count[64] = {0};
   int dev = 0;
@@ -124,7 +140,7 @@ int ensure_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 bool g_dec_smem[4][64], g_decp_smem[4][64], g_pre_smem[4][64], g_prx_smem[4][64], g_tick_smem[64], g_gemm_smem[64], g_argmax_smem[64];
-bool g_sparse_smem[4][64], g_control_smem[64];
+bool g_sparse_smem[4][64], g_control_smem[64], g_w4_smem[6][64];
 
 constexpr int kDefaultOverlapDecodeSms = 100;
 
@@ -195,6 +211,20 @@ int launch_fused_gemm(const typename Epi::Params& p, const CUtensorMap& amap, co
                                    dim3(hb::fused_gemm_threads<Epi>()), smem, stream, p, amap, bmap);
   if (e != cudaSuccess) return fail(HB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
+}
+
+template <int G, int NT>
+int launch_gemm_w4(const hb::GemmW4Params& p, const CUtensorMap& xmap, const CUtensorMap& wmap, int splits,
+                   cudaStream_t stream) {
+  constexpr int slot = (G == 128 ? 0 : G == 64 ? 1 : 2) * 2 + (NT == 128 ? 1 : 0);
+  constexpr int smem = hb::GemmW4Shape<NT>::kSmem;
+  if (int rc = ensure_smem(hb::gemm_w4_kernel<G, NT>, smem, g_w4_smem[slot])) return rc;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const unsigned grid = splits > 1 ? tiles * splits : std::min(tiles, sm_count());
+  const cudaError_t e = launch_cluster(hb::gemm_w4_kernel<G, NT>, dim3(grid), dim3(hb::kW4gThreads), splits, smem, stream,
+                                       p, xmap, wmap);
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "gemm_w4_kernel: %s", cudaGetErrorString(e));
+  return check_launch("gemm_w4_kernel");
 }
 
 // RMSNorm launch: a CTA per row for few rows or hidden beyond 4096, else a warp per row.
@@ -777,6 +807,25 @@ int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const in
     return fail(HB_ERR_INVALID, "4-bit projection pointers must be non-null, x rows and packed 16-byte aligned");
   hb::LinearW4Params p{static_cast<const __nv_bfloat16*>(x), x_stride, reinterpret_cast<const uint32_t*>(packed),
                        static_cast<const __nv_bfloat16*>(scales), zeros, static_cast<__nv_bfloat16*>(out), m, n, k};
+  if (m > 32) {
+    // Smaller groups need more accumulators per step: tiles of 64 tokens.
+    const int tile_tokens = m <= 64 || group != 128 ? 64 : 128;
+    const hb::GemmW4Params g{static_cast<const __nv_bfloat16*>(scales), zeros, static_cast<__nv_bfloat16*>(out), m, n, k,
+                             (m + tile_tokens - 1) / tile_tokens, (n + hb::kW4gRows - 1) / hb::kW4gRows};
+    if (static_cast<int64_t>(g.tiles_m) * g.tiles_n > (1 << 24))
+      return fail(HB_ERR_UNSUPPORTED, "4-bit projection: %d x %d outputs are too many", m, n);
+    CUtensorMap xmap, wmap;
+    if (int rc = encode_2d(&xmap, x, k, m, static_cast<uint64_t>(x_stride) * 2, hb::kW4gBoxK, tile_tokens)) return rc;
+    if (int rc = encode_packed(&wmap, packed, k / 8, n)) return rc;
+    int sms = sm_count();
+    int splits = 1;
+    for (int s = 2; s <= 8 && s * 128 <= k; ++s)
+      if (g.tiles_m * g.tiles_n * s <= sms) splits = s;
+    if (group == 64) return launch_gemm_w4<64, 64>(g, xmap, wmap, splits, stream);
+    if (group == 32) return launch_gemm_w4<32, 64>(g, xmap, wmap, splits, stream);
+    return tile_tokens == 64 ? launch_gemm_w4<128, 64>(g, xmap, wmap, splits, stream)
+                             : launch_gemm_w4<128, 128>(g, xmap, wmap, splits, stream);
+  }
   const int tiles = (n + hb::kW4Rows - 1) / hb::kW4Rows;
   const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
   const int token_tiles = (m + 8 * nt - 1) / (8 * nt);

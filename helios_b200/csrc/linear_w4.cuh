@@ -47,6 +47,7 @@ __device__ __forceinline__ uint32_t cluster_size() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();  // the barrier wants whole warps
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // A float of another CTA's shared memory, at the place `local` has in this CTA's.
@@ -55,6 +56,17 @@ __device__ __forceinline__ float cluster_load(const float* local, uint32_t rank)
   float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float4 cluster_load4(const float* local, uint32_t rank) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
   return v;
 }
 
