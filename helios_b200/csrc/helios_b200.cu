@@ -945,24 +945,27 @@ int hb_control_logits(const void* logits, int64_t row_stride, int32_t rows, int3
   if (logits == nullptr || out == nullptr) return fail(HB_ERR_INVALID, "null logits");
   if (logits == out && row_stride != out_stride) return fail(HB_ERR_INVALID, "in place needs equal row strides");
   if (history != nullptr && (slots == nullptr || lengths == nullptr || prompt_lengths == nullptr || history_rows < 1 ||
-                             history_width < 1 || history_width > INT32_MAX))
+                             history_width < 1))
     return fail(HB_ERR_INVALID, "a history needs its slots, lengths and prompt lengths");
+  if (history != nullptr && history_width > hb::kControlMaxHistory)
+    return fail(HB_ERR_UNSUPPORTED, "histories hold %d tokens at most", hb::kControlMaxHistory);
   if (bias_offsets != nullptr && (bias_entries < 0 || (bias_entries > 0 && (bias_tokens == nullptr || bias_values == nullptr))))
     return fail(HB_ERR_INVALID, "bias offsets need tokens and values");
   if (mask != nullptr && (mask_rows == nullptr || masks < 1)) return fail(HB_ERR_INVALID, "a mask needs its row numbers");
-  unsigned ranks = 8;
-  while (ranks > 1 && vocab <= 1024 * static_cast<int>(ranks)) ranks /= 2;
-  int segment = (vocab + static_cast<int>(ranks) - 1) / static_cast<int>(ranks);
-  segment = std::min((segment + 31) / 32 * 32, hb::kControlMaxSegment);
+  // Few rows take more, smaller segments: about three CTAs per SM.
+  const int fewest = (vocab + hb::kControlMaxSegment - 1) / hb::kControlMaxSegment;
+  const int most_segments = std::max(fewest, vocab / hb::kControlMinSegment);
+  const int segments = std::min(std::max(fewest, 3 * 148 / rows), most_segments);
+  const int segment = ((vocab + segments - 1) / segments + 31) / 32 * 32;
   hb::LogitControlParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<__nv_bfloat16*>(out), row_stride,
                            out_stride, rows, vocab, repetition, frequency, presence, history, history_width,
                            history_rows, slots, lengths, prompt_lengths, bias_offsets, bias_tokens, bias_values, bias_entries,
                            reinterpret_cast<const uint32_t*>(mask), masks, (vocab + 31) / 32, mask_rows, segment};
-  constexpr int most = hb::kControlMaxSegment * 4 + hb::kControlMaxSegment / 8;
+  const int most = hb::control_smem_bytes(hb::kControlMaxSegment, true, true);
   if (int rc = ensure_smem(hb::logit_controls_kernel, most, g_control_smem)) return rc;
-  const cudaError_t e = launch_cluster(hb::logit_controls_kernel, dim3(ranks, rows), dim3(hb::kControlThreads), ranks,
-                                       static_cast<size_t>(segment) * 4 + segment / 8, stream, p);
-  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "logit_controls_kernel: %s", cudaGetErrorString(e));
+  const dim3 grid((vocab + segment - 1) / segment, rows);
+  hb::logit_controls_kernel<<<grid, hb::kControlThreads,
+                              hb::control_smem_bytes(segment, history != nullptr, bias_offsets != nullptr), stream>>>(p);
   return check_launch("logit_controls_kernel");
 }
 

@@ -23,7 +23,14 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# The handle of a device's current stream: what torch.cuda.current_stream(device).cuda_stream
+# gives, without the Stream object (2.2 us of host time per call against 0.06).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
 def _stream(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -217,29 +224,29 @@ def _together(device: torch.device, **tensors: torch.Tensor | None) -> None:
                 raise ValueError(f"{name} must be contiguous")
 
 
-def _call(name: str, device: torch.device, *args) -> None:
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _call(fn, name: str, device: torch.device, *args) -> None:
     """Run an entry point on ``device``'s current stream, with that device current."""
-    fn = getattr(lib(), name)
-    stream = _stream(device)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, stream)
+    if _get_device() == device.index:
+        rc = fn(*args, _stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, stream)
+            rc = fn(*args, _stream(device))
     if rc:
         _native.check(rc, name)
 
 
-def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
-              out: torch.Tensor | None = None) -> torch.Tensor:
-    """``x [m, k] @ W^T`` (bf16 ``[m, n]``) for a weight held in 4 bits: ``W[j, i] = (q[j, i] -
-    z[g, j]) * scales[g, j]``, ``g = i // group``. ``packed`` int32 ``[n, k / 8]`` (word c: even i's
-    in the low half, odd i's in the high half, see hb_linear_w4), ``scales`` bf16 ``[k / group, n]``,
-    ``zeros`` uint8 ``[k / group, n]`` (None: 8); groups of 32, 64 or 128. ``x`` may have any row
-    stride that keeps its rows 16-byte aligned. ``helios_b200.w4.quantize_w4`` makes the three
-    tensors from a weight. Returns ``out``, or a new tensor."""
+# The operators below test their arguments in one expression, which is all that a call in order
+# pays for (each _need costs 0.3 us of host time, more than a decode step's smallest kernels can
+# hide); only when it fails, a second pass finds out which argument to name.
+I32, F32 = torch.int32, torch.float32
+
+
+def _refuse_linear_w4(x, packed, scales, zeros, out) -> None:
     _need(x, BF16, "x", contiguous=False)
-    _need(packed, torch.int32, "packed")
+    _need(packed, I32, "packed")
     _need(scales, BF16, "scales")
     if x.dim() != 2 or packed.dim() != 2 or scales.dim() != 2:
         raise ValueError("x, packed and scales must be 2-D")
@@ -253,16 +260,40 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
         _need(zeros, torch.uint8, "zeros")
         if zeros.shape != scales.shape:
             raise ValueError("zeros must have the shape of scales")
-    dev = x.device
-    if out is None:
-        out = torch.empty((m, n), dtype=BF16, device=dev)
-    else:
+    if out is not None:
         _need(out, BF16, "out")
         if out.shape != (m, n):
             raise ValueError("out must be [m, n]")
-    _together(dev, packed=packed, scales=scales, zeros=zeros, out=out)
-    _call("hb_linear_w4", dev, x.data_ptr(), x.stride(0) if m > 1 else k, m, k, packed.data_ptr(), scales.data_ptr(),
-          _ptr(zeros), n, k // groups, out.data_ptr())
+    _together(x.device, packed=packed, scales=scales, zeros=zeros, out=out)
+    raise ValueError("linear_w4 arguments do not fit together")
+
+
+def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x [m, k] @ W^T`` (bf16 ``[m, n]``) for a weight held in 4 bits: ``W[j, i] = (q[j, i] -
+    z[g, j]) * scales[g, j]``, ``g = i // group``. ``packed`` int32 ``[n, k / 8]`` (word c: even i's
+    in the low half, odd i's in the high half, see hb_linear_w4), ``scales`` bf16 ``[k / group, n]``,
+    ``zeros`` uint8 ``[k / group, n]`` (None: 8); groups of 32, 64 or 128. ``x`` may have any row
+    stride that keeps its rows 16-byte aligned. ``helios_b200.w4.quantize_w4`` makes the three
+    tensors from a weight. Returns ``out``, or a new tensor."""
+    dev = x.device
+    if not (x.is_cuda and x.dtype is BF16 and packed.dtype is I32 and scales.dtype is BF16 and packed.device == dev
+            and scales.device == dev and packed.is_contiguous() and scales.is_contiguous() and x.dim() == 2
+            and packed.dim() == 2 and scales.dim() == 2):
+        _refuse_linear_w4(x, packed, scales, zeros, out)
+    m, k = x.shape
+    n, words = packed.shape
+    groups, scale_n = scales.shape
+    if not (words * 8 == k and scale_n == n and groups and k % groups == 0 and x.stride(1) == 1
+            and (zeros is None or (zeros.dtype is torch.uint8 and zeros.device == dev and zeros.is_contiguous()
+                                   and zeros.shape == scales.shape))
+            and (out is None or (out.dtype is BF16 and out.device == dev and out.is_contiguous()
+                                 and out.shape == (m, n)))):
+        _refuse_linear_w4(x, packed, scales, zeros, out)
+    if out is None:
+        out = x.new_empty((m, n))
+    _call(lib().hb_linear_w4, "hb_linear_w4", dev, x.data_ptr(), x.stride(0) if m > 1 else k, m, k, packed.data_ptr(),
+          scales.data_ptr(), None if zeros is None else zeros.data_ptr(), n, k // groups, out.data_ptr())
     return out
 
 
@@ -272,9 +303,21 @@ BLOCK_KEYS = 64  # keys per block of the sparse attention
 def _check_bounds(key_pool: torch.Tensor, bounds: torch.Tensor) -> None:
     _need(key_pool, BF16, "key_pool")
     _need(bounds, BF16, "bounds")
+    if key_pool.dim() != 4:
+        raise ValueError("key_pool must be [pages, page, kv_heads, head_dim]")
     pages, page, heads, dim = key_pool.shape
     if bounds.shape != (pages, heads, page // BLOCK_KEYS, 2, dim):
         raise ValueError("bounds must be [pages, kv_heads, page / 64, 2, head_dim] for the key pool")
+
+
+def _refuse_bounds(key_pool, bounds, block_table, cu_seq_q, seqused_k, token_row) -> None:
+    _check_bounds(key_pool, bounds)
+    for name, t in (("block_table", block_table), ("cu_seq_q", cu_seq_q), ("seqused_k", seqused_k),
+                    ("token_row", token_row)):
+        _need(t, I32, name)
+    _together(key_pool.device, bounds=bounds, block_table=block_table, cu_seq_q=cu_seq_q, seqused_k=seqused_k,
+              token_row=token_row)
+    raise ValueError("block_table must be [rows, width], with rows + 1 entries in cu_seq_q and rows in seqused_k")
 
 
 def key_block_bounds(key_pool: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor,
@@ -283,20 +326,46 @@ def key_block_bounds(key_pool: torch.Tensor, bounds: torch.Tensor, block_table: 
     ``key_pool [pages, page, Hkv, d]`` and ``bounds [pages, Hkv, page / 64, 2, d]``, with the tick's
     ``block_table [rows, width]``, ``cu_seq_q [rows + 1]``, ``seqused_k [rows]`` and ``token_row
     [tokens]`` (all int32). Only blocks holding new positions are written. Returns ``bounds``."""
-    _check_bounds(key_pool, bounds)
-    for name, t in (("block_table", block_table), ("cu_seq_q", cu_seq_q), ("seqused_k", seqused_k),
-                    ("token_row", token_row)):
-        _need(t, torch.int32, name)
-    rows, width = block_table.shape
-    if cu_seq_q.numel() != rows + 1 or seqused_k.numel() != rows:
-        raise ValueError("cu_seq_q needs rows + 1 entries and seqused_k rows")
     dev = key_pool.device
-    _together(dev, bounds=bounds, block_table=block_table, cu_seq_q=cu_seq_q, seqused_k=seqused_k,
-              token_row=token_row)
-    _call("hb_key_block_bounds", dev, key_pool.data_ptr(), bounds.data_ptr(), key_pool.shape[0], key_pool.shape[1],
+    if not (key_pool.is_cuda and key_pool.dtype is BF16 and bounds.dtype is BF16 and block_table.dtype is I32
+            and cu_seq_q.dtype is I32 and seqused_k.dtype is I32 and token_row.dtype is I32 and bounds.device == dev
+            and block_table.device == dev and cu_seq_q.device == dev and seqused_k.device == dev
+            and token_row.device == dev and key_pool.is_contiguous() and bounds.is_contiguous()
+            and block_table.is_contiguous() and cu_seq_q.is_contiguous() and seqused_k.is_contiguous()
+            and token_row.is_contiguous() and key_pool.dim() == 4 and block_table.dim() == 2):
+        _refuse_bounds(key_pool, bounds, block_table, cu_seq_q, seqused_k, token_row)
+    pages, page, heads, dim = key_pool.shape
+    rows, width = block_table.shape
+    if not (bounds.shape == (pages, heads, page // BLOCK_KEYS, 2, dim) and cu_seq_q.numel() == rows + 1
+            and seqused_k.numel() == rows):
+        _refuse_bounds(key_pool, bounds, block_table, cu_seq_q, seqused_k, token_row)
+    _call(lib().hb_key_block_bounds, "hb_key_block_bounds", dev, key_pool.data_ptr(), bounds.data_ptr(), pages, page,
           block_table.data_ptr(), width, cu_seq_q.data_ptr(), seqused_k.data_ptr(), token_row.data_ptr(), rows,
-          token_row.numel(), key_pool.shape[2], key_pool.shape[3])
+          token_row.numel(), heads, dim)
     return bounds
+
+
+def _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, out, selected, top_blocks) -> None:
+    _need(q, BF16, "q")
+    _need(value_pool, BF16, "value_pool")
+    _check_bounds(key_pool, bounds)
+    _need(block_table, I32, "block_table")
+    _need(seqused_k, I32, "seqused_k")
+    if q.dim() != 3 or value_pool.shape != key_pool.shape or q.shape[2] != key_pool.shape[3]:
+        raise ValueError("q must be [rows, heads, head_dim], and both pools must match each other and its head_dim")
+    if block_table.dim() != 2 or block_table.shape[0] != q.shape[0] or seqused_k.numel() != q.shape[0]:
+        raise ValueError("block_table and seqused_k need one row per query row")
+    if out is not None:
+        _need(out, BF16, "out")
+        if out.shape != q.shape:
+            raise ValueError("out must have the shape of q")
+    if selected is not None:
+        _need(selected, I32, "selected")
+        if selected.shape != (q.shape[0], key_pool.shape[2], top_blocks):
+            raise ValueError("selected must be [rows, kv_heads, top_blocks]")
+    _together(q.device, key_pool=key_pool, value_pool=value_pool, bounds=bounds, block_table=block_table,
+              seqused_k=seqused_k, out=out, selected=selected)
+    raise ValueError("sparse_paged_attention arguments do not fit together")
 
 
 def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, bounds: torch.Tensor,
@@ -305,38 +374,83 @@ def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
                            scale: float | None = None, selected: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one query token per row, ``q [rows, H, d]``, over the ``top_blocks`` 64-key blocks
     that the ``bounds`` of key_block_bounds select for it and each KV head, the row's first
-    ``sink_blocks`` and last ``recent_blocks`` always among them (hb_sparse_paged_attention).
+    ``sink_blocks`` and last ``recent_blocks`` blocks always among them (hb_sparse_paged_attention).
     ``selected`` (int32 ``[rows, Hkv, top_blocks]``) gets the blocks in ascending order, then -1.
     Returns ``out [rows, H, d]``, or a new tensor; a row without keys gives zeros."""
-    _need(q, BF16, "q")
-    _need(value_pool, BF16, "value_pool")
-    _check_bounds(key_pool, bounds)
-    _need(block_table, torch.int32, "block_table")
-    _need(seqused_k, torch.int32, "seqused_k")
+    dev = q.device
+    if not (q.is_cuda and q.dtype is BF16 and key_pool.dtype is BF16 and value_pool.dtype is BF16
+            and bounds.dtype is BF16 and block_table.dtype is I32 and seqused_k.dtype is I32
+            and key_pool.device == dev and value_pool.device == dev and bounds.device == dev
+            and block_table.device == dev and seqused_k.device == dev and q.is_contiguous()
+            and key_pool.is_contiguous() and value_pool.is_contiguous() and bounds.is_contiguous()
+            and block_table.is_contiguous() and seqused_k.is_contiguous() and q.dim() == 3 and key_pool.dim() == 4
+            and block_table.dim() == 2):
+        _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, out, selected, top_blocks)
     rows, heads, dim = q.shape
-    pages, page, kv_heads, pool_dim = key_pool.shape
-    if value_pool.shape != key_pool.shape or dim != pool_dim:
-        raise ValueError("key and value pools must match each other and the query's head_dim")
-    if block_table.dim() != 2 or block_table.shape[0] != rows or seqused_k.numel() != rows:
-        raise ValueError("block_table and seqused_k need one row per query row")
+    pool_shape = key_pool.shape
+    pages, page, kv_heads, pool_dim = pool_shape
+    table_rows, width = block_table.shape
+    if not (value_pool.shape == pool_shape and dim == pool_dim and table_rows == rows and seqused_k.numel() == rows
+            and bounds.shape == (pages, kv_heads, page // BLOCK_KEYS, 2, dim)
+            and (out is None or (out.dtype is BF16 and out.device == dev and out.is_contiguous()
+                                 and out.shape == q.shape))
+            and (selected is None or (selected.dtype is I32 and selected.device == dev and selected.is_contiguous()
+                                      and selected.shape == (rows, kv_heads, top_blocks)))):
+        _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, out, selected, top_blocks)
     if out is None:
         out = torch.empty_like(q)
-    else:
-        _need(out, BF16, "out")
-        if out.shape != q.shape:
-            raise ValueError("out must have the shape of q")
-    if selected is not None:
-        _need(selected, torch.int32, "selected")
-        if selected.shape != (rows, kv_heads, top_blocks):
-            raise ValueError("selected must be [rows, kv_heads, top_blocks]")
-    dev = q.device
-    _together(dev, key_pool=key_pool, value_pool=value_pool, bounds=bounds, block_table=block_table,
-              seqused_k=seqused_k, out=out, selected=selected)
-    _call("hb_sparse_paged_attention", dev, q.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
-          bounds.data_ptr(), pages, page, block_table.data_ptr(), block_table.shape[1], seqused_k.data_ptr(), rows,
-          heads, kv_heads, dim, top_blocks, sink_blocks, recent_blocks, dim ** -0.5 if scale is None else float(scale),
-          _ptr(selected), out.data_ptr())
+    _call(lib().hb_sparse_paged_attention, "hb_sparse_paged_attention", dev, q.data_ptr(), key_pool.data_ptr(),
+          value_pool.data_ptr(), bounds.data_ptr(), pages, page, block_table.data_ptr(), width, seqused_k.data_ptr(),
+          rows, heads, kv_heads, dim, top_blocks, sink_blocks, recent_blocks, dim ** -0.5 if scale is None else scale,
+          None if selected is None else selected.data_ptr(), out.data_ptr())
     return out
+
+
+def _refuse_controls(logits, repetition, frequency, presence, history, slots, lengths, prompt_lengths, bias, mask,
+                     mask_rows, out) -> None:
+    _need(logits, BF16, "logits", contiguous=False)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be [rows, V] with contiguous rows")
+    rows, vocab = logits.shape
+    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        if t is not None:
+            _need(t, F32, name)
+            if t.numel() != rows:
+                raise ValueError(f"{name} needs one value per row")
+    if history is not None:
+        if slots is None or lengths is None or prompt_lengths is None:
+            raise ValueError("a history needs slots, lengths and prompt_lengths")
+        for name, t in (("history", history), ("slots", slots), ("lengths", lengths),
+                        ("prompt_lengths", prompt_lengths)):
+            _need(t, I32, name)
+        if (history.dim() != 2 or slots.numel() != rows or lengths.numel() != history.shape[0]
+                or prompt_lengths.numel() != history.shape[0]):
+            raise ValueError("history must be [slots, width], with one entry of slots per row and of lengths and "
+                             "prompt_lengths per history row")
+    offsets = tokens = values = None
+    if bias is not None:
+        offsets, tokens, values = bias
+        _need(offsets, I32, "bias offsets")
+        _need(tokens, I32, "bias tokens")
+        _need(values, F32, "bias values")
+        if offsets.numel() != rows + 1 or tokens.numel() != values.numel():
+            raise ValueError("bias needs rows + 1 offsets and as many values as tokens")
+    if mask is not None:
+        _need(mask, I32, "mask")
+        if mask_rows is None:
+            raise ValueError("a mask needs mask_rows")
+        _need(mask_rows, I32, "mask_rows")
+        if mask.dim() != 2 or mask.shape[1] != (vocab + 31) // 32 or mask_rows.numel() != rows:
+            raise ValueError("mask must be [masks, ceil(V / 32)] and mask_rows [rows]")
+    if out is not None and out is not logits:
+        _need(out, BF16, "out")
+        if out.shape != logits.shape:
+            raise ValueError("out must have the shape of logits")
+        _together(logits.device, out=out)
+    _together(logits.device, repetition=repetition, frequency=frequency, presence=presence, history=history,
+              slots=slots, lengths=lengths, prompt_lengths=prompt_lengths, bias_offsets=offsets, bias_tokens=tokens,
+              bias_values=values, mask=mask, mask_rows=mask_rows)
+    raise ValueError("control_logits arguments do not fit together")
 
 
 def control_logits(logits: torch.Tensor, *, repetition: torch.Tensor | None = None,
@@ -353,60 +467,52 @@ def control_logits(logits: torch.Tensor, *, repetition: torch.Tensor | None = No
     slot -1: none). ``bias``: int32 offsets ``[rows + 1]``, int32 tokens (ascending within a row) and
     fp32 values. ``mask`` int32 ``[masks, ceil(V / 32)]`` with ``mask_rows`` int32 ``[rows]`` (-1: none).
     Returns ``out`` (``logits`` itself works in place), or a new tensor."""
-    _need(logits, BF16, "logits", contiguous=False)
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise ValueError("logits must be [rows, V] with contiguous rows")
-    rows, vocab = logits.shape
     dev = logits.device
-    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-        if t is not None:
-            _need(t, torch.float32, name)
-            if t.numel() != rows:
-                raise ValueError(f"{name} needs one value per row")
-    history_rows = history_width = 0
+    args = (repetition, frequency, presence, history, slots, lengths, prompt_lengths, bias, mask, mask_rows, out)
+    if not (logits.is_cuda and logits.dtype is BF16 and logits.dim() == 2 and logits.stride(1) == 1):
+        _refuse_controls(logits, *args)
+    rows, vocab = logits.shape
+    for t in (repetition, frequency, presence):
+        if t is not None and not (t.dtype is F32 and t.device == dev and t.numel() == rows and t.is_contiguous()):
+            _refuse_controls(logits, *args)
+    history_rows = history_width = entries = masks = 0
+    history_ptrs = bias_ptrs = (None, None, None, None)
+    mask_ptr = mask_rows_ptr = None
     if history is not None:
-        if slots is None or lengths is None or prompt_lengths is None:
-            raise ValueError("a history needs slots, lengths and prompt_lengths")
-        for name, t in (("history", history), ("slots", slots), ("lengths", lengths),
-                        ("prompt_lengths", prompt_lengths)):
-            _need(t, torch.int32, name)
-        if history.dim() != 2:
-            raise ValueError("history must be [slots, width]")
+        if slots is None or lengths is None or prompt_lengths is None or history.dim() != 2:
+            _refuse_controls(logits, *args)
         history_rows, history_width = history.shape
-        if slots.numel() != rows or lengths.numel() != history_rows or prompt_lengths.numel() != history_rows:
-            raise ValueError("slots needs one entry per row, lengths and prompt_lengths one per history row")
-    offsets = tokens = values = None
+        if not (history.dtype is I32 and slots.dtype is I32 and lengths.dtype is I32 and prompt_lengths.dtype is I32
+                and history.device == dev and slots.device == dev and lengths.device == dev
+                and prompt_lengths.device == dev and history.is_contiguous() and slots.is_contiguous()
+                and lengths.is_contiguous() and prompt_lengths.is_contiguous() and slots.numel() == rows
+                and lengths.numel() == history_rows and prompt_lengths.numel() == history_rows):
+            _refuse_controls(logits, *args)
+        history_ptrs = (history.data_ptr(), slots.data_ptr(), lengths.data_ptr(), prompt_lengths.data_ptr())
     if bias is not None:
         offsets, tokens, values = bias
-        _need(offsets, torch.int32, "bias offsets")
-        _need(tokens, torch.int32, "bias tokens")
-        _need(values, torch.float32, "bias values")
-        if offsets.numel() != rows + 1 or tokens.numel() != values.numel():
-            raise ValueError("bias needs rows + 1 offsets and as many values as tokens")
-    masks = 0
+        entries = tokens.numel()
+        if not (offsets.dtype is I32 and tokens.dtype is I32 and values.dtype is F32 and offsets.device == dev
+                and tokens.device == dev and values.device == dev and offsets.is_contiguous()
+                and tokens.is_contiguous() and values.is_contiguous() and offsets.numel() == rows + 1
+                and values.numel() == entries):
+            _refuse_controls(logits, *args)
+        bias_ptrs = (offsets.data_ptr(), tokens.data_ptr(), values.data_ptr())
     if mask is not None:
-        _need(mask, torch.int32, "mask")
-        if mask_rows is None:
-            raise ValueError("a mask needs mask_rows")
-        _need(mask_rows, torch.int32, "mask_rows")
-        masks = mask.shape[0]
-        if mask.dim() != 2 or mask.shape[1] != (vocab + 31) // 32 or mask_rows.numel() != rows:
-            raise ValueError("mask must be [masks, ceil(V / 32)] and mask_rows [rows]")
+        if not (mask_rows is not None and mask.dtype is I32 and mask_rows.dtype is I32 and mask.device == dev
+                and mask_rows.device == dev and mask.is_contiguous() and mask_rows.is_contiguous()
+                and mask.dim() == 2 and mask.shape[1] == (vocab + 31) // 32 and mask_rows.numel() == rows):
+            _refuse_controls(logits, *args)
+        masks, mask_ptr, mask_rows_ptr = mask.shape[0], mask.data_ptr(), mask_rows.data_ptr()
     if out is None:
-        out = torch.empty((rows, vocab), dtype=BF16, device=dev)
-    elif out is not logits:
-        _need(out, BF16, "out")
-        if out.shape != logits.shape or out.device != dev:
-            raise ValueError("out must have the shape and device of logits")
-    _together(dev, repetition=repetition, frequency=frequency, presence=presence, history=history, slots=slots,
-              lengths=lengths, prompt_lengths=prompt_lengths, bias_offsets=offsets, bias_tokens=tokens,
-              bias_values=values, mask=mask, mask_rows=mask_rows)
-    wide = rows > 1
-    _call("hb_control_logits", dev, logits.data_ptr(), logits.stride(0) if wide else vocab, rows, vocab,
-          _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(history), history_rows, history_width, _ptr(slots),
-          _ptr(lengths), _ptr(prompt_lengths), _ptr(offsets), _ptr(tokens), _ptr(values),
-          0 if tokens is None else tokens.numel(), _ptr(mask), masks,
-          _ptr(mask_rows), out.data_ptr(), out.stride(0) if wide else vocab)
+        out = logits.new_empty((rows, vocab))
+    elif out is not logits and not (out.dtype is BF16 and out.device == dev and out.shape == logits.shape
+                                    and out.is_contiguous()):
+        _refuse_controls(logits, *args)
+    _call(lib().hb_control_logits, "hb_control_logits", dev, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+          rows, vocab, _ptr(repetition), _ptr(frequency), _ptr(presence), history_ptrs[0], history_rows,
+          history_width, history_ptrs[1], history_ptrs[2], history_ptrs[3], bias_ptrs[0], bias_ptrs[1], bias_ptrs[2],
+          entries, mask_ptr, masks, mask_rows_ptr, out.data_ptr(), out.stride(0) if rows > 1 else vocab)
     return out
 
 

@@ -297,7 +297,8 @@ HB_API int hb_sparse_paged_attention(const void* q, const void* key_pool, const 
  * presence; a listed token gains its bias; a token the row's mask does not allow becomes -inf.
  * The result is rounded once to bf16. Each control may be null.
  *   history         int32 [history_rows][history_width]; row r uses row slots[r] (-1: none), its
- *                   first lengths[slot] entries, of which the first prompt_lengths[slot] are prompt
+ *                   first lengths[slot] entries, of which the first prompt_lengths[slot] are prompt;
+ *                   history_width at most 65,535
  *   bias_offsets    int32 [rows + 1] into bias_tokens / bias_values [bias_entries]; tokens ascend within a row,
  *                   of equal neighbours the last counts, a token followed by a smaller one is
  *                   skipped and flagged (HB_STATUS_BAD_TOKEN)

@@ -58,7 +58,7 @@ def test_logit_control_refusals(lib):
     assert call(stride=99) == invalid and call(out_stride=99) == invalid and call(vocab=0) == invalid
     assert call(rows=70_000) == invalid and call(logits=None) == invalid
     assert call(history=P) == invalid and "history" in _native.last_error()
-    assert call(history=P, slots=P, width=2 ** 31) == invalid
+    assert call(history=P, slots=P, width=65_536) == _native.HB_ERR_UNSUPPORTED
     assert call(offsets=P, entries=3) == invalid and call(offsets=P, entries=-1) == invalid
     assert call(mask=P, masks=1) == invalid
     assert call(out=P, stride=100, out_stride=104) == invalid and "in place" in _native.last_error()
