@@ -99,6 +99,8 @@ struct SparseAttentionParams {
   const int32_t* seqused_k;     // [rows]
   int32_t* selected;            // [rows, kv_heads, top] or null
   int32_t width, num_pages, page_size, heads, kv_heads;
+  int32_t per_page;        // blocks per page
+  uint32_t per_page_inv;   // ceil(2^32 / per_page), 0 for one block per page
   int32_t top, sink, recent;
   float scale_log2;
 };
@@ -130,21 +132,40 @@ __device__ __forceinline__ void cluster_store(uint32_t* local, uint32_t rank, ui
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 
-// The bounds of block b for KV head h, or null where the table names no page.
-__device__ __forceinline__ const __nv_bfloat16* block_bounds(const SparseAttentionParams& p, int row, int h, int b) {
-  const int per_page = p.page_size / kBlockKeys;
-  const int pidx = b / per_page;
-  const int page = p.block_table[static_cast<int64_t>(row) * p.width + pidx];
-  if (page < 0 || page >= p.num_pages) return nullptr;
-  return p.bounds + ((static_cast<int64_t>(page) * p.kv_heads + h) * per_page + b % per_page) * 256;
+// b / per_page, exact for b x per_page < 2^32.
+__device__ __forceinline__ int block_page(const SparseAttentionParams& p, int b) {
+  return p.per_page_inv ? static_cast<int>(__umulhi(static_cast<uint32_t>(b), p.per_page_inv)) : b;
 }
 
-// Scores of blocks [b0, b1) (b0 a multiple of 8) into keys[], by the CTA's warps; returns the
+// The bounds of block b for KV head h, or null where the row's pages (shared memory) name none.
+__device__ __forceinline__ const __nv_bfloat16* block_bounds(const SparseAttentionParams& p, const int* pages, int h,
+                                                             int b) {
+  const int pidx = block_page(p, b), page = pages[pidx];
+  if (page < 0 || page >= p.num_pages) return nullptr;
+  return p.bounds + ((static_cast<int64_t>(page) * p.kv_heads + h) * p.per_page + (b - pidx * p.per_page)) * 256;
+}
+
+// Scores of blocks [b0, b1) (b0 a multiple of 8) into the keys[] of every CTA of the cluster (0
+// for the first `sink` and, from block `last`, the forced ones), by the CTA's warps; returns the
 // lane's largest sum |terms|.
 template <int GROUP>
-__device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, int row, int h, int b0, int b1,
-                                              uint32_t* keys, int ranks) {
+__device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, const int* pages, int row, int h, int b0,
+                                              int b1, int last, uint32_t* keys, int ranks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, c4 = lane & 3;
+  float worst = 0.f;
+  // Two groups' bounds are on their way while one is multiplied.
+  auto load = [&](int base, uint4 (&v)[8]) {
+    const int b = base + g4;
+    const __nv_bfloat16* src = b < b1 ? block_bounds(p, pages, h, b) : nullptr;
+    if (b < b1 && src == nullptr) raise_status(kStatusBadPage);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = src ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c4) : make_uint4(0, 0, 0, 0);
+  };
+  constexpr int kStep = 8 * kSparseWarps;
+  uint4 even[8], odd[8];
+  load(b0 + 8 * warp, even);
+  load(b0 + 8 * warp + kStep, odd);
   // Query fragments: head g4, dims 32 j + 8 c4 .. + 7; the negative part, then the positive.
   uint32_t qn[4][4], qp[4][4];
 #pragma unroll
@@ -163,27 +184,23 @@ __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, in
       qp[j][i] = *reinterpret_cast<const uint32_t*>(&m);
     }
   }
-  float worst = 0.f;
-  for (int base = b0 + 8 * warp; base < b1; base += 8 * kSparseWarps) {
-    const int b = base + g4;
-    const __nv_bfloat16* src = b < b1 ? block_bounds(p, row, h, b) : nullptr;
-    if (b < b1 && src == nullptr) raise_status(kStatusBadPage);
-    uint4 v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = src ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c4) : make_uint4(0, 0, 0, 0);
-    float s[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (ranks > 1) cluster_wait();  // every CTA of the cluster has started
+  auto multiply = [&](int base, const uint4 (&v)[8]) {
+    // Two chains each for the scores and for sum |terms|: a warp MMA's result is 30 cycles away.
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr uint32_t kAbs = 0x7FFF7FFFu;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t* q = j < 4 ? qn[j & 3] : qp[j & 3];
       const uint32_t f0[4] = {q[0], 0u, q[1], 0u}, f1[4] = {q[2], 0u, q[3], 0u};
-      mma_16816(s, f0, v[j].x, v[j].y);
-      mma_16816(s, f1, v[j].z, v[j].w);
+      mma_16816(s0, f0, v[j].x, v[j].y);
+      mma_16816(s1, f1, v[j].z, v[j].w);
       const uint32_t e0[4] = {q[0] & kAbs, 0u, q[1] & kAbs, 0u}, e1[4] = {q[2] & kAbs, 0u, q[3] & kAbs, 0u};
-      mma_16816(a, e0, v[j].x & kAbs, v[j].y & kAbs);
-      mma_16816(a, e1, v[j].z & kAbs, v[j].w & kAbs);
+      mma_16816(a0, e0, v[j].x & kAbs, v[j].y & kAbs);
+      mma_16816(a1, e1, v[j].z & kAbs, v[j].w & kAbs);
     }
+    const float s[2] = {s0[0] + s1[0], s0[1] + s1[1]}, a[2] = {a0[0] + a1[0], a0[1] + a1[1]};
     // Head g4, blocks base + 2 c4 and + 1: the largest over the group's heads.
     uint32_t k0 = g4 < GROUP ? score_key(s[0]) : 0u, k1 = g4 < GROUP ? score_key(s[1]) : 0u;
 #pragma unroll
@@ -193,11 +210,19 @@ __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, in
     }
     const float big = fmaxf(a[0], a[1]);
     worst = (a[0] < INFINITY && a[1] < INFINITY) ? fmaxf(worst, big) : INFINITY;
-    // Lane (g4, c4) hands the pair to CTA g4 (+ 8 for clusters beyond 8).
-    for (int r = g4; r < ranks; r += 8) {
-      if (base + 2 * c4 < b1) cluster_store(keys + base + 2 * c4, r, k0);
-      if (base + 2 * c4 + 1 < b1) cluster_store(keys + base + 2 * c4 + 1, r, k1);
-    }
+    // Lane (g4, c4) hands the pair to CTA g4.
+    const int e0 = base + 2 * c4, e1 = e0 + 1;
+    if (e0 < p.sink || e0 >= last) k0 = 0u;
+    if (e1 < p.sink || e1 >= last) k1 = 0u;
+    if (g4 < ranks && e0 < b1) cluster_store(keys + e0, g4, k0);
+    if (g4 < ranks && e1 < b1) cluster_store(keys + e1, g4, k1);
+  };
+  for (int base = b0 + 8 * warp; base < b1; base += 2 * kStep) {
+    multiply(base, even);
+    load(base + 2 * kStep, even);
+    if (base + kStep >= b1) break;
+    multiply(base + kStep, odd);
+    load(base + 3 * kStep, odd);
   }
   return worst;
 }
@@ -206,8 +231,8 @@ struct SparseShared {
   uint64_t full[kDecStages], empty[kDecStages];
   int abort_flag;
   uint32_t worst;  // largest sum |terms| (float bits; the CTAs' maxima meet here)
-  int n_border, n_in, n_sel, digit, remaining;
-  uint32_t hist[256];
+  int n_border;
+  int taken[kSparseWarps];
   float merge_ml[kDecConsumerWarps][16][2];
   float part[8][128];     // unnormalised output of each head of the group over this CTA's blocks
   float part_ml[8][2];    // its running maximum and sum
@@ -215,9 +240,9 @@ struct SparseShared {
 
 // Exact score of block b (see the head of this file) by a whole warp, as an ordered integer.
 template <int GROUP>
-__device__ unsigned long long exact_score(const SparseAttentionParams& p, int row, int h, int b) {
+__device__ unsigned long long exact_score(const SparseAttentionParams& p, const int* pages, int row, int h, int b) {
   const int lane = threadIdx.x & 31;
-  const __nv_bfloat16* src = block_bounds(p, row, h, b);
+  const __nv_bfloat16* src = block_bounds(p, pages, h, b);
   unsigned long long best = 0ull;
   if (src == nullptr) return best;
   const uint2 lo2 = *reinterpret_cast<const uint2*>(src + 4 * lane);
@@ -243,100 +268,99 @@ __device__ unsigned long long exact_score(const SparseAttentionParams& p, int ro
   return best;
 }
 
-// Turns keys[0 .. nb) into 1 (taken) or 0, with `need` of the blocks [sink, nb - recent) taken;
-// every thread of the CTA calls it. `index` and `score` are scratch for the blocks near the cut.
-template <int GROUP>
-__device__ void select_blocks(const SparseAttentionParams& p, int row, int h, int nb, int need, uint32_t* keys,
-                              uint32_t* index, unsigned long long* score, SparseShared& sh) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int c0 = p.sink, c1 = nb - p.recent;  // need <= c1 - c0, see the caller
-  uint32_t prefix = 0, known = 0;             // the cut's leading bits so far
-  int remaining = need;
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSparseThreads) sh.hist[i] = 0u;
-      __syncthreads();
-      for (int b = c0 + tid; b < c1; b += kSparseThreads)
-        if ((keys[b] & known) == prefix) atomicAdd(&sh.hist[(keys[b] >> shift) & 255u], 1u);
-      __syncthreads();
-      if (warp == 0) {  // bins from the top: lane l has 255 - 8 l .. 248 - 8 l
-        uint32_t sum = 0;
+// A threshold on keys[] such that the keys above it are those of the `need` (>= 1) best blocks
+// with non-zero keys; keys[] is padded with zeros to a multiple of 128. Every warp finds the
+// need-th largest key for itself, by bisection: the scores of one row differ in their low 20 bits
+// or so. With at most 128 KEEP keys (KEEP > 0) a lane holds its keys in registers. Only where the
+// computed scores near the cut do not settle it do the warps work together: the keys there are
+// replaced by the largest or the smallest one, by exact score (`index` and `score` are scratch).
+template <int GROUP, int KEEP>
+__device__ uint32_t cut_blocks(const SparseAttentionParams& p, const int* pages, int row, int h, int nb, int need,
+                               float worst, uint32_t* keys, uint32_t* index, unsigned long long* score,
+                               int* n_border) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint4* k4 = reinterpret_cast<const uint4*>(keys) + lane;
+  const int passes = KEEP > 0 ? KEEP : (nb + 127) / 128;
+  uint4 kept[KEEP > 0 ? KEEP : 1];
+  if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += sh.hist[255 - 8 * lane - i];
-        uint32_t incl = sum;
+    for (int i = 0; i < KEEP; ++i) kept[i] = 128 * i < nb ? k4[32 * i] : make_uint4(0, 0, 0, 0);
+  }
+  // f for every four keys of the lane, or for each of them.
+  auto each4 = [&](auto f) {
+    if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += v;
-        }
-        uint32_t before = incl - sum;
-        if (before < static_cast<uint32_t>(remaining) && static_cast<uint32_t>(remaining) <= incl) {
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t n = sh.hist[255 - 8 * lane - i];
-            if (static_cast<uint32_t>(remaining) <= before + n) {
-              sh.digit = 255 - 8 * lane - i;
-              sh.remaining = remaining - static_cast<int>(before);
-              break;
-            }
-            before += n;
-          }
-        }
+      for (int i = 0; i < KEEP; ++i) f(kept[i].x, kept[i].y, kept[i].z, kept[i].w);
+    } else {
+      for (int i = 0; i < passes; ++i) {
+        const uint4 v = k4[32 * i];
+        f(v.x, v.y, v.z, v.w);
       }
-      __syncthreads();
-      prefix |= static_cast<uint32_t>(sh.digit) << shift;
-      known |= 255u << shift;
-      remaining = sh.remaining;
-      __syncthreads();
+    }
+  };
+  auto each = [&](auto f) {
+    each4([&](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+      f(a);
+      f(b);
+      f(c);
+      f(d);
+    });
+  };
+  uint32_t hi = 0u, lo = 0xFFFFFFFFu;
+  each([&](uint32_t k) {
+    hi = max(hi, k);
+    lo = min(lo, k - 1u);  // 0 wraps to the largest
+  });
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  lo = __reduce_min_sync(0xffffffffu, lo) + 1u;
+  bool met = false;  // exactly `need` keys reach lo; always: count(key >= lo) >= need > count(key > hi)
+  while (lo < hi && !met) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;  // lo < mid <= hi
+    int n = 0;
+    each4([&](uint32_t a, uint32_t b, uint32_t c, uint32_t d) { n += ((a >= mid) + (b >= mid)) + ((c >= mid) + (d >= mid)); });
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (n >= need) {
+      lo = mid;
+      met = n == need;
+    } else {
+      hi = mid - 1;
     }
   }
-  // prefix is the need-th largest computed score.
-  const float eps2 = 2.f * 3.0517578125e-5f * __uint_as_float(sh.worst);  // 2 eps, eps = 2^-15 sum |terms|
-  const float cut = key_score(prefix);
-  uint32_t low = 0u, high = 0xFFFFFFFFu;  // every block between them (NaN included) is scored again
-  bool all = true;
-  if (eps2 < INFINITY && fabsf(cut) < INFINITY && prefix != 0xFFFFFFFFu) {
-    // One more step outwards for the rounding of these two sums.
+  uint32_t kth = 0xFFFFFFFFu;  // the need-th largest key
+  each([&](uint32_t k) { kth = min(kth, k >= lo ? k : 0xFFFFFFFFu); });
+  kth = __reduce_min_sync(0xffffffffu, kth);
+  const float eps2 = 2.f * 3.0517578125e-5f * worst;  // 2 eps, eps = 2^-15 sum |terms|
+  const float cut = key_score(kth);
+  // Every block within 2 eps of the cut (all of them where scores are not finite), one more step
+  // outwards for the rounding of these sums.
+  uint32_t low = 1u, high = 0xFFFFFFFFu;
+  if (eps2 < INFINITY && fabsf(cut) < INFINITY && kth != 0xFFFFFFFFu) {
     low = score_key(__fsub_rd(cut, eps2));
     high = score_key(__fadd_ru(cut, eps2));
-    all = false;
   }
-  if (tid == 0) sh.n_border = sh.n_in = 0;
+  int count = 0;  // keys above the border, and in its low half those in it
+  each([&](uint32_t k) { count += k > high ? 0x10000 : k >= low ? 1 : 0; });  // low >= 1: never a forced block
+  count = __reduce_add_sync(0xffffffffu, count);
+  const int left = need - (count >> 16), border = count & 0xFFFF;
+  if (left >= border) return low - 1u;  // all of them: no doubt
+  // The same decision in every warp: the CTA goes on together.
+  for (int b = threadIdx.x; b < nb; b += kSparseThreads)
+    if (keys[b] >= low && keys[b] <= high) index[atomicAdd(n_border, 1)] = static_cast<uint32_t>(b);
   __syncthreads();
-  int in = 0;
-  for (int b = c0 + tid; b < c1; b += kSparseThreads) {
-    const uint32_t k = keys[b];
-    if (need <= 0 || (!all && k < low)) {
-      keys[b] = 0u;
-    } else if (!all && k > high) {
-      keys[b] = 1u;
-      ++in;
-    } else {
-      keys[b] = 0u;
-      index[atomicAdd(&sh.n_border, 1)] = static_cast<uint32_t>(b);
-    }
-  }
-  for (int b = tid; b < c0; b += kSparseThreads) keys[b] = 1u;
-  for (int b = c1 + tid; b < nb; b += kSparseThreads) keys[b] = 1u;
-  if (in) atomicAdd(&sh.n_in, in);
-  __syncthreads();
-  const int border = sh.n_border, left = need - sh.n_in;
-  if (left >= border) {  // all of them
-    for (int i = tid; i < border; i += kSparseThreads) keys[index[i]] = 1u;
-  } else if (left > 0) {
-    for (int i = warp; i < border; i += kSparseWarps) {
-      const unsigned long long s = exact_score<GROUP>(p, row, h, static_cast<int>(index[i]));
-      if (lane == 0) score[i] = s;
-    }
-    __syncthreads();
-    for (int i = tid; i < border; i += kSparseThreads) {
-      const unsigned long long s = score[i];
-      const uint32_t b = index[i];
-      int rank = 0;
-      for (int j = 0; j < border; ++j) rank += score[j] > s || (score[j] == s && index[j] < b);
-      if (rank < left) keys[b] = 1u;
-    }
+  for (int i = warp; i < border; i += kSparseWarps) {
+    const unsigned long long s = exact_score<GROUP>(p, pages, row, h, static_cast<int>(index[i]));
+    if (lane == 0) score[i] = s;
   }
   __syncthreads();
+  for (int i = threadIdx.x; i < border; i += kSparseThreads) {  // the larger score, then the lower block
+    const unsigned long long s = score[i];
+    const uint32_t b = index[i];
+    int rank = 0;
+    for (int j = 0; j < border; ++j) rank += score[j] > s || (score[j] == s && index[j] < b);
+    keys[b] = rank < left ? 0xFFFFFFFFu : 1u;
+  }
+  __syncthreads();
+  return min(high, 0xFFFFFFFEu);
 }
 
 // One cluster per (row, KV head): its CTAs score a share of the row's blocks each and hand the
@@ -355,12 +379,13 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
   unsigned long long* score = reinterpret_cast<unsigned long long*>(index + kSparseMaxBlocks);
   int* list = reinterpret_cast<int*>(smem + kDecRingBytes);  // [top] selected blocks, ascending
   int* where = list + p.top;                                 // [top] first pool token, -1: no page
+  int* pages = where + p.top;                                // [width] the row's pages
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
   const int h = blockIdx.y, row = blockIdx.z;
-  const int per_page = p.page_size / kBlockKeys;
   int len = p.seqused_k[row];
+  for (int i = tid; i < p.width; i += kSparseThreads) pages[i] = p.block_table[static_cast<int64_t>(row) * p.width + i];
   if (len > p.width * p.page_size) {  // more keys than the table has pages for
     if (tid == 0 && rank == 0) raise_status(kStatusBadPage);
     len = p.width * p.page_size;
@@ -373,15 +398,19 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
     }
     sh.abort_flag = 0;
     sh.worst = 0u;
+    sh.n_border = 0;
     fence_barrier_init();
   }
   const bool choose = nb > p.top;  // row-uniform: the whole cluster agrees
-  if (choose) {
-    if (ranks > 1) cluster_sync();  // every CTA of the cluster has started and set its words
-    else __syncthreads();
-    const int groups = (nb + 7) / 8;
+  const int need = choose ? p.top - p.sink - p.recent : 0;
+  uint32_t above = 0u;  // blocks with keys above this are taken, and the forced ones
+  __syncthreads();
+  if (need > 0) {
+    if (ranks > 1) cluster_arrive();  // the words that the others write are set
+    const int last = nb - p.recent, groups = (nb + 7) / 8;
     const int b0 = 8 * (groups * rank / ranks), b1 = min(nb, 8 * (groups * (rank + 1) / ranks));
-    float worst = score_blocks<GROUP>(p, row, h, b0, b1, keys, ranks);
+    for (int b = nb + tid; b < (nb + 127) / 128 * 128; b += kSparseThreads) keys[b] = 0u;
+    float worst = score_blocks<GROUP>(p, pages, row, h, b0, b1, last, keys, ranks);
     worst = warp_max(worst);
     if (lane < ranks) {  // non-negative floats compare as their bits do
       uint32_t a;
@@ -390,28 +419,52 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
     }
     if (ranks > 1) cluster_sync();
     else __syncthreads();
-    select_blocks<GROUP>(p, row, h, nb, p.top - p.sink - p.recent, keys, index, score, sh);
+    const float size = __uint_as_float(sh.worst);
+    above = nb <= 640 ? cut_blocks<GROUP, 5>(p, pages, row, h, nb, need, size, keys, index, score, &sh.n_border)
+                      : cut_blocks<GROUP, 0>(p, pages, row, h, nb, need, size, keys, index, score, &sh.n_border);
   }
-  if (warp == 0) {  // ascending list
-    int n = 0;
-    for (int b0 = 0; b0 < nb; b0 += 32) {
-      const int b = b0 + lane;
-      const bool take = b < nb && (!choose || keys[b] != 0u);
-      const unsigned m = __ballot_sync(0xffffffffu, take);
-      const int at = n + __popc(m & ((1u << lane) - 1u));
-      if (take && at < p.top) list[at] = b;
-      n += __popc(m);
+  // Ascending list: four blocks per thread at a time, places by a scan over the CTA.
+  int n_sel = 0;
+  if (!choose) {
+    n_sel = nb;
+    for (int i = tid; i < nb; i += kSparseThreads) list[i] = i;
+  } else {
+    for (int b0 = 0; b0 < nb; b0 += 4 * kSparseThreads) {
+      const int b = b0 + 4 * tid;
+      uint32_t take = 0;
+      uint4 k = make_uint4(0, 0, 0, 0);
+      if (need > 0 && b < nb) k = *reinterpret_cast<const uint4*>(keys + b);
+      const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        take |= (b + e < nb && (w[e] > above || b + e < p.sink || b + e >= nb - p.recent) ? 1u : 0u) << e;
+      const int mine = __popc(take);
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) sh.taken[warp] = incl;
+      __syncthreads();
+      int at = n_sel + incl - mine;
+#pragma unroll
+      for (int x = 0; x < kSparseWarps; ++x) {
+        if (x < warp) at += sh.taken[x];
+        n_sel += sh.taken[x];
+      }
+      for (; take; take &= take - 1, ++at)
+        if (at < p.top) list[at] = b + __ffs(take) - 1;
+      __syncthreads();
     }
-    if (lane == 0) sh.n_sel = min(n, p.top);  // min(nb, top)
+    n_sel = min(n_sel, p.top);  // it is p.top
   }
   __syncthreads();
-  const int n_sel = sh.n_sel;
   for (int i = tid; i < n_sel; i += kSparseThreads) {
-    const int b = list[i];
-    const int page = p.block_table[static_cast<int64_t>(row) * p.width + b / per_page];
+    const int b = list[i], pidx = block_page(p, b), page = pages[pidx];
     const bool ok = page >= 0 && page < p.num_pages;
     if (!ok) raise_status(kStatusBadPage);
-    where[i] = ok ? page * p.page_size + (b % per_page) * kBlockKeys : -1;
+    where[i] = ok ? page * p.page_size + (b - pidx * p.per_page) * kBlockKeys : -1;
   }
   if (p.selected != nullptr && rank == 0) {
     int32_t* dst = p.selected + (static_cast<int64_t>(row) * p.kv_heads + h) * p.top;
@@ -504,13 +557,27 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
   // (den is 0 then alone: a NaN or infinite score leaves den NaN, and shows).
   for (int i = rank * kSparseThreads + tid; i < GROUP * 128; i += ranks * kSparseThreads) {
     const int g = i / 128, d = i % 128;
+    float m[8], l[8], v[8];  // every CTA's parts are asked for before any is used
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (r < ranks) {
+        m[r] = cluster_load(&sh.part_ml[g][0], r);
+        l[r] = cluster_load(&sh.part_ml[g][1], r);
+        v[r] = cluster_load(&sh.part[g][d], r);
+      }
+    }
     float mx = -INFINITY, num = 0.f, den = 0.f;
-    for (int r = 0; r < ranks; ++r) mx = fmaxf(mx, cluster_load(&sh.part_ml[g][0], r));
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < ranks) mx = fmaxf(mx, m[r]);
     const float base = mx == -INFINITY ? 0.f : mx;
-    for (int r = 0; r < ranks; ++r) {
-      const float w = exp2f(cluster_load(&sh.part_ml[g][0], r) - base);
-      num += w * cluster_load(&sh.part[g][d], r);
-      den += w * cluster_load(&sh.part_ml[g][1], r);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (r < ranks) {
+        const float w = exp2f(m[r] - base);
+        num += w * v[r];
+        den += w * l[r];
+      }
     }
     p.out[(static_cast<int64_t>(row) * p.heads + h * GROUP + g) * 128 + d] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
   }

@@ -905,13 +905,15 @@ int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* v
     return rc;
   if (int rc = encode_3d(&vmap, value_pool, head_dim, kv_heads, pool_tokens, head_dim * 2, row_bytes, 64, 1, hb::kBlockKeys))
     return rc;
+  const int per_page = page_size / hb::kBlockKeys;
   hb::SparseAttentionParams p{static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out),
                               static_cast<const __nv_bfloat16*>(bounds), block_table, seqused_k, selected, width,
-                              static_cast<int32_t>(num_pages), page_size, heads, kv_heads, top_blocks, sink_blocks,
-                              recent_blocks, scale * 1.4426950408889634f};
+                              static_cast<int32_t>(num_pages), page_size, heads, kv_heads, per_page,
+                              per_page > 1 ? static_cast<uint32_t>(((1ull << 32) + per_page - 1) / per_page) : 0u,
+                              top_blocks, sink_blocks, recent_blocks, scale * 1.4426950408889634f};
   const int gs = group_slot(group);
-  const size_t smem = hb::kDecSmemBytes + 8 * static_cast<size_t>(top_blocks);
-  const int most = hb::kDecSmemBytes + 8 * hb::kSparseMaxTop;
+  const size_t smem = hb::kDecSmemBytes + 8 * static_cast<size_t>(top_blocks) + 4 * static_cast<size_t>(width);
+  const int most = hb::kDecSmemBytes + 8 * hb::kSparseMaxTop + 4 * hb::kSparseMaxBlocks;
   int ranks = 1;
   while (ranks < 8 && 2 * ranks <= top_blocks && static_cast<int64_t>(num_rows) * kv_heads * ranks * 2 <= 2 * 148) ranks *= 2;
   const dim3 grid(ranks, kv_heads, num_rows);

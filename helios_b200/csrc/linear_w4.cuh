@@ -50,6 +50,15 @@ __device__ __forceinline__ void cluster_sync() {
   __syncwarp();  // the barrier wants whole warps
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of cluster_sync, for work in between (each thread once, in this order).
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // A float of another CTA's shared memory, at the place `local` has in this CTA's.
 __device__ __forceinline__ float cluster_load(const float* local, uint32_t rank) {
   uint32_t a;
