@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
   constexpr int kStepMmas = kW4gStepK / 16;
   constexpr int GPS = kW4gStepK / G;                  // groups per step, one accumulator each
   constexpr int kLag = Shape::kAccs / GPS;            // steps until a step's accumulators come round again
-  static_assert(kLag >= 1 && kLag <= S, "a step's accumulators");
+  static_assert(kLag >= 1 && S % kLag == 0, "a step's accumulators");
   extern __shared__ __align__(1024) uint8_t dsm[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
   uint8_t* packed = smem;
@@ -208,23 +208,32 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
     const uint64_t desc0 = smem_desc(smem_u32(xs), 16, 1024, kSwizzle128B);
     const int mine = first_tile < tiles ? (tiles - first_tile + tile_step - 1) / tile_step : 0;
     const int total = mine * steps;  // steps of all this CTA's tiles
-    bool seen = false;               // the step's barrier was found complete during the step before
+    bool seen = false, ok = true;    // seen: the step's barrier was found complete during the step before
+    // Unrolled over the ring, so that descriptors and tensor-memory addresses are constants beside
+    // a uniform base.
 #pragma unroll 1
-    for (int it = 0; it < total; ++it) {
-      const int st = it % S;
-      if (!seen && !mbar_wait_fast(&ready[st], (it / S) & 1, &abort_flag)) break;
-      tc_fence_after();
-      seen = mbar_poll(&ready[(it + 1) % S], ((it + 1) / S) & 1);
-      const uint64_t b = desc0 + static_cast<uint64_t>((st * Shape::kXBytes) >> 4);
-      const uint32_t a = tmem_a + kW4gACols * st;
-      const uint32_t d = tmem + (it % kLag) * (GPS * NT);
-      // Past k's end the codes and activations are zeros: whole groups of them, never added.
+    for (int it0 = 0; ok && it0 < total; it0 += S) {
+      const uint32_t parity = (it0 / S) & 1;
 #pragma unroll
-      for (int j = 0; j < kStepMmas; ++j)
-        mma_ts_warp(d + (j / kGroupMmas) * NT, a + 8 * j,
-                    b + (j / 4) * static_cast<uint64_t>(Shape::kBoxBytes >> 4) + 2 * (j % 4), idesc,
-                    j % kGroupMmas != 0 ? 1u : 0u);
-      mma_commit_warp(&done[st]);
+      for (int st = 0; st < S; ++st) {
+        if (it0 + st >= total) break;
+        if (!seen && !mbar_wait_fast(&ready[st], parity, &abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        seen = mbar_poll(&ready[(st + 1) % S], st + 1 < S ? parity : parity ^ 1u);
+        const uint64_t b = desc0 + static_cast<uint64_t>((st * Shape::kXBytes) >> 4);
+        const uint32_t a = tmem_a + kW4gACols * st;
+        const uint32_t d = tmem + (st % kLag) * (GPS * NT);  // S is a multiple of kLag
+        // Past k's end the codes and activations are zeros: whole groups of them, never added.
+#pragma unroll
+        for (int j = 0; j < kStepMmas; ++j)
+          mma_ts_warp(d + (j / kGroupMmas) * NT, a + 8 * j,
+                      b + (j / 4) * static_cast<uint64_t>(Shape::kBoxBytes >> 4) + 2 * (j % 4), idesc,
+                      j % kGroupMmas != 0 ? 1u : 0u);
+        mma_commit_warp(&done[st]);
+      }
     }
     mma_commit_warp(&drain_bar);  // nothing may still write tensor memory when it is freed
     mbar_drain(&drain_bar, 0);

@@ -100,13 +100,13 @@ int encode_2d(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, 
   return HB_OK;
 }
 
-// 2-D map over packed 4-bit weights, int32 [rows][words]: box (32 words, 128 rows), 128-byte swizzle.
-int encode_packed(CUtensorMap* map, const void* base, uint64_t words, uint64_t rows) {
+// 2-D map over packed 4-bit weights, int32 [rows][words]: box (32 words, box_rows rows), 128-byte swizzle.
+int encode_packed(CUtensorMap* map, const void* base, uint64_t words, uint64_t rows, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(HB_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[2] = {words, rows};
   const cuuint64_t strides[1] = {words * 4};
-  const cuuint32_t box[2] = {hb::kW4gPackedK / 8, hb::kW4gRows};
+  const cuuint32_t box[2] = {hb::kW4gPackedK / 8, box_rows};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
@@ -140,7 +140,7 @@ int ensure_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 bool g_dec_smem[4][64], g_decp_smem[4][64], g_pre_smem[4][64], g_prx_smem[4][64], g_tick_smem[64], g_gemm_smem[64], g_argmax_smem[64];
-bool g_sparse_smem[4][64], g_control_smem[64], g_w4_smem[6][64];
+bool g_sparse_smem[4][64], g_control_smem[64], g_w4_smem[6][64], g_w4s_smem[18][64];
 
 constexpr int kDefaultOverlapDecodeSms = 100;
 
@@ -211,6 +211,19 @@ int launch_fused_gemm(const typename Epi::Params& p, const CUtensorMap& amap, co
                                    dim3(hb::fused_gemm_threads<Epi>()), smem, stream, p, amap, bmap);
   if (e != cudaSuccess) return fail(HB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
+}
+
+template <int G, int NT, bool ZEROS>
+int launch_linear_w4(const hb::LinearW4Params& p, const CUtensorMap& xmap, const CUtensorMap& wmap, dim3 grid,
+                     cudaStream_t stream) {
+  constexpr int slot = ((G == 128 ? 0 : G == 64 ? 1 : 2) * 3 + (NT == 4 ? 2 : NT - 1)) * 2 + (ZEROS ? 1 : 0);
+  constexpr int smem = hb::W4Stage<NT>::kSmem;
+  if (int rc = ensure_smem(hb::linear_w4_kernel<G, NT, ZEROS>, smem, g_w4s_smem[slot])) return rc;
+  const cudaError_t e =
+      launch_cluster(hb::linear_w4_kernel<G, NT, ZEROS>, grid, dim3(hb::kW4Threads), grid.x, smem, stream, p,
+                                       xmap, wmap);
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "linear_w4_kernel: %s", cudaGetErrorString(e));
+  return check_launch("linear_w4_kernel");
 }
 
 template <int G, int NT>
@@ -816,7 +829,7 @@ int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const in
       return fail(HB_ERR_UNSUPPORTED, "4-bit projection: %d x %d outputs are too many", m, n);
     CUtensorMap xmap, wmap;
     if (int rc = encode_2d(&xmap, x, k, m, static_cast<uint64_t>(x_stride) * 2, hb::kW4gBoxK, tile_tokens)) return rc;
-    if (int rc = encode_packed(&wmap, packed, k / 8, n)) return rc;
+    if (int rc = encode_packed(&wmap, packed, k / 8, n, hb::kW4gRows)) return rc;
     int sms = sm_count();
     int splits = 1;
     for (int s = 2; s <= 8 && s * 128 <= k; ++s)
@@ -826,29 +839,34 @@ int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const in
     return tile_tokens == 64 ? launch_gemm_w4<128, 64>(g, xmap, wmap, splits, stream)
                              : launch_gemm_w4<128, 128>(g, xmap, wmap, splits, stream);
   }
-  const int tiles = (n + hb::kW4Rows - 1) / hb::kW4Rows;
   const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
-  const int token_tiles = (m + 8 * nt - 1) / (8 * nt);
-  if (token_tiles > 65535) return fail(HB_ERR_UNSUPPORTED, "4-bit projection: too many token rows (%d)", m);
+  const int tiles = (n + hb::kW4Rows - 1) / hb::kW4Rows, token_tiles = (m + 8 * nt - 1) / (8 * nt);
+  // K splits, where one wave of CTAs holds them (with some room, as clusters do not fill every SM):
+  // the fewest that share the stages out as evenly as any.
+  const int stages = (k + hb::kW4StageK - 1) / hb::kW4StageK;
+  const int64_t wave = 148 * (nt == 1 ? hb::W4Stage<1>::kPerSm : nt == 2 ? hb::W4Stage<2>::kPerSm : hb::W4Stage<4>::kPerSm);
   int splits = 1;
-  while (splits < 4 && static_cast<int64_t>(tiles) * token_tiles * splits < 2 * 148 && k / (splits * 2) >= 1024) splits *= 2;
-  cudaError_t e = cudaSuccess;
-#define HB_W4_LAUNCH(G, NT)                                                                                \
-  e = launch_cluster(hb::linear_w4_kernel<G, NT>, dim3(splits, tiles, token_tiles), dim3(32 * hb::kW4Warps), \
-                     splits, 0, stream, p)
-#define HB_W4_GROUP(G)                  \
-  do {                                  \
-    if (nt == 1) HB_W4_LAUNCH(G, 1);    \
-    else if (nt == 2) HB_W4_LAUNCH(G, 2); \
-    else HB_W4_LAUNCH(G, 4);            \
+  for (int s = 2; s <= hb::kW4MaxSplits; ++s)
+    if (static_cast<int64_t>(tiles) * token_tiles * s * 10 <= wave * 9 && (stages + s - 1) / s < (stages + splits - 1) / splits)
+      splits = s;
+  const dim3 grid(splits, tiles, token_tiles);
+  CUtensorMap xmap, wmap;
+  if (int rc = encode_2d(&xmap, x, k, m, static_cast<uint64_t>(x_stride) * 2, 64, 8 * nt)) return rc;
+  if (int rc = encode_packed(&wmap, packed, k / 8, n, hb::kW4Rows)) return rc;
+#define HB_W4_ZEROS(G, NT) \
+  return zeros != nullptr ? launch_linear_w4<G, NT, true>(p, xmap, wmap, grid, stream) \
+                          : launch_linear_w4<G, NT, false>(p, xmap, wmap, grid, stream)
+#define HB_W4_GROUP(G)                 \
+  do {                                 \
+    if (nt == 1) HB_W4_ZEROS(G, 1);    \
+    if (nt == 2) HB_W4_ZEROS(G, 2);    \
+    HB_W4_ZEROS(G, 4);                 \
   } while (0)
   if (group == 128) HB_W4_GROUP(128);
-  else if (group == 64) HB_W4_GROUP(64);
-  else HB_W4_GROUP(32);
+  if (group == 64) HB_W4_GROUP(64);
+  HB_W4_GROUP(32);
 #undef HB_W4_GROUP
-#undef HB_W4_LAUNCH
-  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "linear_w4_kernel: %s", cudaGetErrorString(e));
-  return check_launch("linear_w4_kernel");
+#undef HB_W4_ZEROS
 }
 
 int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_pages, int32_t page_size,

@@ -5,16 +5,26 @@
 // q is 0..15; z is 8 where no zero points are given. The weight is read as it is stored:
 // packed int32 [N, K / 8], word j of a row holding k = 8j .. 8j + 7 with the even k's in its low
 // 16 bits and the odd k's in its high 16 bits, four bits each in ascending k, so
-// (word >> 4i) & 0x000F000F is the pair k = 8j + 2i, 8j + 2i + 1. OR-ing 0x4300 into each half
-// makes the bf16 values 128 + q, and subtracting 128 + z (also a bf16 value) is exact, so two
-// weights cost one LOP3 and one packed subtraction.
+// (word >> 4i) & 0x000F000F is the pair k = 8j + 2i, 8j + 2i + 1, and OR-ing 0x4300 into each half
+// makes the bf16 values 128 + q: two weights for a shift and a LOP3. The MMAs multiply these; the
+// sum of a group's activations comes from one more MMA row of ones, and the group's products are
+//   sum (q - z) x = sum (128 + q) x - (128 + z) sum x
+// in fp32, whose rounding there is 2^-24 of at most 143 sum |x|: some 40 times that of
+// sum |q - z| |x| itself and still 2^11 below the bf16 output's. (Subtracting 128 + z from every
+// weight first, exactly, cost a third of the instructions that this path is bound by.)
 //
 // Products run on m16n8k16 warp MMAs with 16 weight rows as M and 8 tokens as N. The sum over k
 // does not depend on which k a fragment register holds, as long as A and B agree, so a thread
-// takes its k's as consecutive words of the packed row (one 16-byte load per row for groups of
-// 128) and its activations as the matching 16-byte loads: no reordering on either side. A
-// group's products are summed in a fresh fp32 accumulator and scaled once, in fp32, so the only
-// rounding to bf16 is the output's.
+// takes its k's as consecutive words of the packed row (16 bytes per row for groups of 128) and
+// its activations as the matching 16-byte pieces: no reordering on either side. Every group is
+// summed in a fresh fp32 accumulator and scaled once, in fp32, so the only rounding to bf16 is the
+// output's.
+//
+// A CTA has 64 weight rows, two warps for every 16, and all tokens of its tile. One more brings weights
+// and activations by TMA into a ring of stages of 256 k's, so that every SM keeps 190 KB and more
+// on the way whatever the others do. (One token, 19456 x 2560: 14.5 us with each warp loading its
+// own fragments, 13.9 with 16-byte asynchronous copies by all threads, 18.2 with bulk copies of
+// single rows.) A cluster of CTAs shares k where there are few weight rows.
 #pragma once
 
 #include "hb_common.cuh"
@@ -31,10 +41,23 @@ struct LinearW4Params {
   int32_t m, n, k;
 };
 
-constexpr int kW4Warps = 8;
-constexpr int kW4Rows = 16;   // weight rows per CTA (the MMA M)
-constexpr int kW4Chunk = 128;  // k's a warp takes at a time
-constexpr int kW4Batch = 2;   // chunks whose loads are issued before any is used
+constexpr int kW4Tiles = 4;             // MMA tiles of 16 weight rows per CTA
+constexpr int kW4Halves = 2;            // warps per tile, taking the two halves of every stage's k's
+constexpr int kW4Warps = kW4Tiles * kW4Halves;
+constexpr int kW4Threads = 32 * (kW4Warps + 1);  // and the copying one
+constexpr int kW4Rows = 16 * kW4Tiles;  // weight rows per CTA
+constexpr int kW4StageK = 256;          // k's per stage: 128 bytes of a packed row
+constexpr int kW4MaxSplits = 8;
+
+template <int NT>
+struct W4Stage {
+  static constexpr int kWeightBytes = kW4Rows * kW4StageK / 2;  // one box of 128-byte rows
+  static constexpr int kBoxBytes = 8 * NT * 128;                // activations: a box per 64 k's
+  static constexpr int kBytes = kWeightBytes + kW4StageK / 64 * kBoxBytes;
+  static constexpr int kStages = NT == 1 ? 5 : NT == 2 ? 4 : 3;
+  static constexpr int kSmem = kStages * kBytes + 1024;  // 61, 65 and 73 KB
+  static constexpr int kPerSm = NT == 1 ? 3 : 2;         // CTAs that fit an SM, by registers
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -90,142 +113,205 @@ __device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t zz, uint32_t (&p)
   }
 }
 
-// One warp's share of the products of 16 weight rows (row0 ..) with 8 NT tokens (t0 ..): chunks
-// first, first + step, ... of 128 k's, into acc (the MMA's C layout: rows lane / 4 and + 8,
-// tokens 8 nt + 2 (lane % 4) and + 1).
-template <int G, int NT>
-__device__ __forceinline__ void w4_rows(const LinearW4Params& p, int row0, int t0, int first, int step,
-                                        float (&acc)[NT][4]) {
-  constexpr int WPG = G / 32;        // words of one group that a thread holds
-  constexpr int GPC = kW4Chunk / G;  // groups per chunk
-  const int lane = threadIdx.x & 31, g4 = lane >> 2, c4 = lane & 3;
-  const int chunks = (p.k + kW4Chunk - 1) / kW4Chunk, words = p.k / 8;
-  const int ra = row0 + g4, rb = ra + 8;
-  const bool ok_a = ra < p.n, ok_b = rb < p.n;
-  const uint32_t* wa = p.packed + static_cast<int64_t>(ok_a ? ra : 0) * words;
-  const uint32_t* wb = p.packed + static_cast<int64_t>(ok_b ? rb : 0) * words;
-  for (int c0 = first; c0 < chunks; c0 += step * kW4Batch) {
-    uint32_t qa[kW4Batch][4], qb[kW4Batch][4];
-    float sa[kW4Batch][GPC], sb[kW4Batch][GPC];
-    uint32_t za[kW4Batch][GPC], zb[kW4Batch][GPC];
+template <int WORDS>
+__device__ __forceinline__ void shared_load(uint32_t src, uint32_t (&v)[WORDS]) {
+  if constexpr (WORDS == 4)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src));
+  else if constexpr (WORDS == 2)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(src));
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(src));
+}
+// Grid (cluster of K splits, row tiles, token tiles). Rank r of a cluster has the stages r, r +
+// splits, ...; the CTAs' sums are added in rank order, from shared memory, so results do not
+// depend on timing. Weight rows, tokens and k's past the end arrive as zeros.
+template <int G, int NT, bool ZEROS>
+__global__ void __launch_bounds__(kW4Threads, W4Stage<NT>::kPerSm) linear_w4_kernel(LinearW4Params p, const __grid_constant__ CUtensorMap xmap,
+                                                               const __grid_constant__ CUtensorMap wmap) {
+  using Stage = W4Stage<NT>;
+  constexpr int WPG = G / 32;         // words of one group that a thread holds
+  constexpr int GPT = kW4StageK / G / kW4Halves;  // groups per stage and warp
+  constexpr int kTokens = 8 * NT, kStages = Stage::kStages;
+  extern __shared__ __align__(1024) uint8_t dsm[];
+  const uint32_t ring = (smem_u32(dsm) + 1023u) & ~1023u;
+  // The sums, once the ring is idle: [token][row].
+  constexpr int kPartStride = kW4Rows + 4;
+  static_assert(kTokens * kPartStride * 4 <= Stage::kSmem - 1024, "the sums fit the ring");
+  float* parts = reinterpret_cast<float*>(dsm + (ring - smem_u32(dsm)));
+  __shared__ uint64_t full[kStages], empty[kStages];
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, c4 = lane & 3;
+  const int splits = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+  const int row0 = blockIdx.y * kW4Rows, t0 = blockIdx.z * kTokens;
+  const int all = (p.k + kW4StageK - 1) / kW4StageK;
+  const int n = rank < all ? (all - rank + splits - 1) / splits : 0;  // this CTA's stages
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kW4Warps);
+    }
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+
+  float acc[NT][4];
 #pragma unroll
-    for (int b = 0; b < kW4Batch; ++b) {
-      const int c = c0 + b * step;
+  for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+  if (warp == kW4Warps) {
+    if (lane == 0) {
+      int s = 0;
+      for (; s < n; ++s) {
+        const int st = s % kStages, k0 = (rank + s * splits) * kW4StageK;
+        if (s >= kStages && !mbar_wait(&empty[st], ((s / kStages) - 1) & 1, &abort_flag)) break;
+        const uint32_t dst = ring + st * Stage::kBytes;
+        mbar_expect_tx(&full[st], Stage::kBytes);
+        tma_load_2d_at(dst, &wmap, &full[st], k0 / 8, row0);
 #pragma unroll
-      for (int gi = 0; gi < GPC; ++gi) {
-        const int k0 = c * kW4Chunk + gi * G;
-        const bool in = k0 < p.k;  // k is a multiple of G: a group is there whole or not at all
-        const int word = k0 / 8 + c4 * WPG;
-        sa[b][gi] = sb[b][gi] = 0.f;
-        za[b][gi] = zb[b][gi] = 0x43084308u;
+        for (int b = 0; b < kW4StageK / 64; ++b)
+          tma_load_2d_at(dst + Stage::kWeightBytes + b * Stage::kBoxBytes, &xmap, &full[st], k0 + 64 * b, t0);
+      }
+      for (int j = max(0, s - kStages); j < s; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
+    }
+    __syncwarp();
+  } else {
+    // Scales and zero points of this thread's rows, two stages ahead in registers (DRAM is further
+    // away than one). Past k's end any scale does.
+    const int tile = warp % kW4Tiles, half = warp / kW4Tiles;
+    const int ra = min(row0 + 16 * tile + g4, p.n - 1), rb = min(row0 + 16 * tile + g4 + 8, p.n - 1);
+    const int groups = p.k / G;
+    struct Scales {
+      __nv_bfloat16 a[GPT], b[GPT];
+      uint8_t za[GPT], zb[GPT];
+    };
+    auto load_scales = [&](int s, Scales& v) {
+      const int first = ((rank + s * splits) * kW4Halves + half) * GPT;
 #pragma unroll
-        for (int i = 0; i < WPG; ++i) qa[b][gi * WPG + i] = qb[b][gi * WPG + i] = 0u;
-        if (in && ok_a) {
-          if constexpr (WPG == 4) {
-            *reinterpret_cast<uint4*>(&qa[b][0]) = __ldg(reinterpret_cast<const uint4*>(wa + word));
-          } else if constexpr (WPG == 2) {
-            *reinterpret_cast<uint2*>(&qa[b][gi * 2]) = __ldg(reinterpret_cast<const uint2*>(wa + word));
-          } else {
-            qa[b][gi] = __ldg(wa + word);
-          }
-        }
-        if (in && ok_b) {
-          if constexpr (WPG == 4) {
-            *reinterpret_cast<uint4*>(&qb[b][0]) = __ldg(reinterpret_cast<const uint4*>(wb + word));
-          } else if constexpr (WPG == 2) {
-            *reinterpret_cast<uint2*>(&qb[b][gi * 2]) = __ldg(reinterpret_cast<const uint2*>(wb + word));
-          } else {
-            qb[b][gi] = __ldg(wb + word);
-          }
-        }
-        if (in) {
-          const int64_t at = static_cast<int64_t>(k0 / G) * p.n;
-          if (ok_a) sa[b][gi] = __bfloat162float(p.scales[at + ra]);
-          if (ok_b) sb[b][gi] = __bfloat162float(p.scales[at + rb]);
-          if (p.zeros != nullptr) {
-            if (ok_a) za[b][gi] = (0x4300u | (p.zeros[at + ra] & 15u)) * 0x00010001u;
-            if (ok_b) zb[b][gi] = (0x4300u | (p.zeros[at + rb] & 15u)) * 0x00010001u;
-          }
+      for (int g = 0; g < GPT; ++g) {
+        const int64_t at = static_cast<int64_t>(min(first + g, groups - 1)) * p.n;
+        v.a[g] = p.scales[at + ra];
+        v.b[g] = p.scales[at + rb];
+        if (ZEROS) {
+          v.za[g] = p.zeros[at + ra];
+          v.zb[g] = p.zeros[at + rb];
         }
       }
-    }
+    };
+    Scales now, next;
+    load_scales(0, now);
+    load_scales(1, next);
+    const uint32_t wfrag = ring + 128 * (16 * tile + g4);
+    // The half's activations start two boxes on.
+    const uint32_t xfrag = ring + Stage::kWeightBytes + half * (kW4StageK / 64 / kW4Halves) * Stage::kBoxBytes + 128 * g4;
+    for (int s = 0; s < n; ++s) {
+      const int st = s % kStages;
+      float fa[GPT], fb[GPT], oa[GPT], ob[GPT];  // scales and 128 + zero points
 #pragma unroll
-    for (int b = 0; b < kW4Batch; ++b) {
-      const int c = c0 + b * step;
-      if (c >= chunks) break;
+      for (int g = 0; g < GPT; ++g) {
+        fa[g] = __bfloat162float(now.a[g]);
+        fb[g] = __bfloat162float(now.b[g]);
+        oa[g] = ZEROS ? 128.f + (now.za[g] & 15) : 136.f;
+        ob[g] = ZEROS ? 128.f + (now.zb[g] & 15) : 136.f;
+      }
+      now = next;
+      load_scales(s + 2, next);
+      if (!mbar_wait_fast(&full[st], (s / kStages) & 1, &abort_flag)) break;
+      const uint32_t wst = wfrag + st * Stage::kBytes, xst = xfrag + st * Stage::kBytes;
 #pragma unroll
-      for (int gi = 0; gi < GPC; ++gi) {
-        const int k0 = c * kW4Chunk + gi * G + c4 * 8 * WPG;
-        float part[NT][4];
+      for (int g = 0; g < GPT; ++g) {
+        // Rows 16 tile + g4 and + 8 (the same swizzle): 4 WPG bytes from 64 half + g G / 2 + 4 WPG c4.
+        uint32_t qa[WPG], qb[WPG];
+        const int piece = 4 * half + g * (G / 32) + (WPG == 4 ? c4 : WPG == 2 ? c4 >> 1 : 0);
+        const int within = WPG == 4 ? 0 : WPG == 2 ? (c4 & 1) * 8 : c4 * 4;
+        shared_load<WPG>(wst + ((piece ^ g4) << 4) + within, qa);
+        shared_load<WPG>(wst + ((piece ^ g4) << 4) + within + 8 * 128, qb);
+        float part[NT][4], ones[NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
+        for (int t = 0; t < NT; ++t) {
+          part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
+          ones[t][0] = ones[t][1] = ones[t][2] = ones[t][3] = 0.f;
+        }
 #pragma unroll
-        for (int i = 0; i < WPG; ++i) {
-          uint32_t pa[4], pb[4];
-          w4_unpack(qa[b][gi * WPG + i], za[b][gi], pa);
-          w4_unpack(qb[b][gi * WPG + i], zb[b][gi], pb);
-          const uint32_t a0[4] = {pa[0], pb[0], pa[1], pb[1]}, a1[4] = {pa[2], pb[2], pa[3], pb[3]};
+        for (int w = 0; w < WPG; ++w) {
+          constexpr uint32_t kOne = 0x3F803F80u;
+          constexpr uint32_t one[4] = {kOne, kOne, kOne, kOne};
+          uint32_t a[4], b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a[e] = ((qa[w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
+            b[e] = ((qb[w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
+          }
+          const uint32_t a0[4] = {a[0], b[0], a[1], b[1]}, a1[4] = {a[2], b[2], a[3], b[3]};
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const int token = t0 + 8 * t + g4, k = k0 + 8 * i;
-            uint4 xv = make_uint4(0, 0, 0, 0);
-            if (token < p.m && k < p.k) xv = *reinterpret_cast<const uint4*>(p.x + token * p.x_stride + k);
-            mma_16816(part[t], a0, xv.x, xv.y);
-            mma_16816(part[t], a1, xv.z, xv.w);
+            uint32_t x[4];
+            const int at = g * (G / 8) + WPG * c4 + w;  // 16-byte piece of the half's 16
+            shared_load<4>(xst + (at >> 3) * Stage::kBoxBytes + (((at & 7) ^ g4) << 4) + 8 * 128 * t, x);
+            mma_16816(part[t], a0, x[0], x[1]);
+            mma_16816(ones[t], one, x[0], x[1]);
+            mma_16816(part[t], a1, x[2], x[3]);
+            mma_16816(ones[t], one, x[2], x[3]);
           }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          acc[t][0] += sa[b][gi] * part[t][0];
-          acc[t][1] += sa[b][gi] * part[t][1];
-          acc[t][2] += sb[b][gi] * part[t][2];
-          acc[t][3] += sb[b][gi] * part[t][3];
+          acc[t][0] += fa[g] * (part[t][0] - oa[g] * ones[t][0]);
+          acc[t][1] += fa[g] * (part[t][1] - oa[g] * ones[t][1]);
+          acc[t][2] += fb[g] * (part[t][2] - ob[g] * ones[t][2]);
+          acc[t][3] += fb[g] * (part[t][3] - ob[g] * ones[t][3]);
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
     }
-  }
-}
-
-// Grid (cluster of K splits, row tiles, token tiles). The chunks of a row go round the cluster's
-// warps; a CTA sums its warps' parts in warp order, rank 0 the CTAs' in rank order (from their
-// shared memory), so results do not depend on timing.
-template <int G, int NT>
-__global__ void __launch_bounds__(32 * kW4Warps) linear_w4_kernel(LinearW4Params p) {
-  __shared__ float parts[kW4Warps][NT * 8][kW4Rows];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, c4 = lane & 3;
-  const int splits = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
-  const int row0 = blockIdx.y * kW4Rows, t0 = blockIdx.z * (8 * NT);
-  float acc[NT][4];
+    named_barrier_sync(1, 32 * kW4Warps);  // every warp has read its last stage
+    if (half == 1) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-  w4_rows<G, NT>(p, row0, t0, rank * kW4Warps + warp, splits * kW4Warps, acc);
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    parts[warp][8 * t + 2 * c4][g4] = acc[t][0];
-    parts[warp][8 * t + 2 * c4 + 1][g4] = acc[t][1];
-    parts[warp][8 * t + 2 * c4][g4 + 8] = acc[t][2];
-    parts[warp][8 * t + 2 * c4 + 1][g4 + 8] = acc[t][3];
-  }
-  __syncthreads();
-  constexpr int kOut = NT * 8 * kW4Rows;
-  float* mine = &parts[0][0][0];
-  for (int i = threadIdx.x; i < kOut; i += 32 * kW4Warps) {
-    float s = mine[i];
+        for (int e = 0; e < 4; ++e) parts[(8 * t + 2 * c4 + (e & 1)) * kPartStride + 16 * tile + g4 + 8 * (e >> 1)] = acc[t][e];
+    }
+    named_barrier_sync(1, 32 * kW4Warps);
+    if (half == 0) {
 #pragma unroll
-    for (int w = 1; w < kW4Warps; ++w) s += mine[w * kOut + i];
-    mine[i] = s;
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) parts[(8 * t + 2 * c4 + (e & 1)) * kPartStride + 16 * tile + g4 + 8 * (e >> 1)] += acc[t][e];
+    }
+    __syncwarp();
   }
   if (splits > 1) cluster_sync();
   else __syncthreads();
-  if (rank == 0) {
-    for (int i = threadIdx.x; i < kOut; i += 32 * kW4Warps) {
-      const int token = t0 + i / kW4Rows, row = row0 + i % kW4Rows;
-      float s = mine[i];
-      for (int r = 1; r < splits; ++r) s += cluster_load(mine + i, r);
-      if (token < p.m && row < p.n) p.out[static_cast<int64_t>(token) * p.n + row] = __float2bfloat16_rn(s);
+  const int tokens = min(kTokens, p.m - t0);
+  // Every CTA finishes a share of the outputs, four rows at a time.
+  const bool wide = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
+  for (int i = rank * kW4Threads + tid; i < tokens * kW4Rows / 4; i += splits * kW4Threads) {
+    const int token = i / (kW4Rows / 4), r = 4 * (i % (kW4Rows / 4)), row = row0 + r;
+    if (row >= p.n) continue;
+    float4 v[kW4MaxSplits];
+#pragma unroll
+    for (int q = 0; q < kW4MaxSplits; ++q)
+      if (q < splits) v[q] = cluster_load4(parts + token * kPartStride + r, q);
+    float4 s = v[0];
+#pragma unroll
+    for (int q = 1; q < kW4MaxSplits; ++q)
+      if (q < splits) {
+        s.x += v[q].x;
+        s.y += v[q].y;
+        s.z += v[q].z;
+        s.w += v[q].w;
+      }
+    const float o[4] = {s.x, s.y, s.z, s.w};
+    __nv_bfloat16* dst = p.out + static_cast<int64_t>(t0 + token) * p.n + row;
+    if (wide) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (row + e < p.n) dst[e] = __float2bfloat16_rn(o[e]);
     }
   }
-  if (splits > 1) cluster_sync();  // the other CTAs' shared memory stays until rank 0 has read it
+  if (splits > 1) cluster_sync();  // the sums stay until every CTA has read them
 }
 
 }  // namespace hb
