@@ -8,6 +8,7 @@ ops raise when the library is missing or the tensors are not on a CUDA device.
 """
 
 from helios_b200.config import Qwen3Config, Sampling, qwen3_4b_config
+from helios_b200.controls import LogitControls, TokenHistory
 from helios_b200.paged_cache import (
     KVPage,
     KVPagePool,
@@ -15,6 +16,7 @@ from helios_b200.paged_cache import (
     PagedBatchCache,
     PagedKVBlockSnapshot,
     PagedKVCache,
+    SparseAttention,
 )
 
 __all__ = [
@@ -24,7 +26,10 @@ __all__ = [
     "PagedBatchCache",
     "PagedKVBlockSnapshot",
     "PagedKVCache",
+    "LogitControls",
     "Qwen3Config",
     "Sampling",
+    "SparseAttention",
+    "TokenHistory",
     "qwen3_4b_config",
 ]

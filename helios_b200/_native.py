@@ -63,7 +63,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "hb_lm_head_argmax": (c_int, [P, I32, I32, P, I32, P, P, P]),
     "hb_linear_w4": (c_int, [P, I64, I32, I32, P, P, P, I32, I32, P, P]),
     "hb_key_block_bounds": (c_int, [P, P, I64, I32, P, I32, P, P, P, I32, I32, I32, I32, P]),
-    "hb_sparse_paged_attention": (c_int, [P, P, P, P, I64, I32, P, I32, P, I32, I32, I32, I32, I32, I32, I32, F32, P,
+    "hb_sparse_paged_attention": (c_int, [P, P, P, P, I64, I32, P, I32, P, P, I32, I32, I32, I32, I32, I32, I32, F32, P,
                                           P, P]),
     "hb_control_logits": (c_int, [P, I64, I32, I32, P, P, P, P, I32, I64, P, P, P, P, P, P, I32, P, I32, P, P, I64, P]),
     "hb_embedding": (c_int, [P, P, I64, P, I64, I32, P]),

@@ -92,11 +92,12 @@ __global__ void __launch_bounds__(kBoundsThreads) key_block_bounds_kernel(BlockB
 
 // ---------------------------------------------------------------- selection and attention
 struct SparseAttentionParams {
-  const __nv_bfloat16* q;       // [rows, H, 128]
-  __nv_bfloat16* out;           // [rows, H, 128]
+  const __nv_bfloat16* q;       // [tokens, H, 128]
+  __nv_bfloat16* out;           // [tokens, H, 128]
   const __nv_bfloat16* bounds;  // [num_pages, kv_heads, page_size / 64, 2, 128]
   const int32_t* block_table;   // [rows, width]
   const int32_t* seqused_k;     // [rows]
+  const int32_t* cu_seq_q;      // [rows + 1]: rows with other than one token are left alone; null: row r has token r
   int32_t* selected;            // [rows, kv_heads, top] or null
   int32_t width, num_pages, page_size, heads, kv_heads;
   int32_t per_page;        // blocks per page
@@ -149,7 +150,7 @@ __device__ __forceinline__ const __nv_bfloat16* block_bounds(const SparseAttenti
 // for the first `sink` and, from block `last`, the forced ones), by the CTA's warps; returns the
 // lane's largest sum |terms|.
 template <int GROUP>
-__device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, const int* pages, int row, int h, int b0,
+__device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, const int* pages, int token, int h, int b0,
                                               int b1, int last, uint32_t* keys, int ranks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, c4 = lane & 3;
   float worst = 0.f;
@@ -172,7 +173,7 @@ __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, co
   for (int j = 0; j < 4; ++j) {
     uint4 v = make_uint4(0, 0, 0, 0);
     if (g4 < GROUP)
-      v = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(row) * p.heads + h * GROUP + g4) * 128 + 32 * j +
+      v = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(token) * p.heads + h * GROUP + g4) * 128 + 32 * j +
                                           8 * c4);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
@@ -240,7 +241,7 @@ struct SparseShared {
 
 // Exact score of block b (see the head of this file) by a whole warp, as an ordered integer.
 template <int GROUP>
-__device__ unsigned long long exact_score(const SparseAttentionParams& p, const int* pages, int row, int h, int b) {
+__device__ unsigned long long exact_score(const SparseAttentionParams& p, const int* pages, int token, int h, int b) {
   const int lane = threadIdx.x & 31;
   const __nv_bfloat16* src = block_bounds(p, pages, h, b);
   unsigned long long best = 0ull;
@@ -250,7 +251,7 @@ __device__ unsigned long long exact_score(const SparseAttentionParams& p, const 
   const __nv_bfloat16 *lo = reinterpret_cast<const __nv_bfloat16*>(&lo2), *hi = reinterpret_cast<const __nv_bfloat16*>(&hi2);
 #pragma unroll 1
   for (int g = 0; g < GROUP; ++g) {
-    const uint2 q2 = *reinterpret_cast<const uint2*>(p.q + (static_cast<int64_t>(row) * p.heads + h * GROUP + g) * 128 + 4 * lane);
+    const uint2 q2 = *reinterpret_cast<const uint2*>(p.q + (static_cast<int64_t>(token) * p.heads + h * GROUP + g) * 128 + 4 * lane);
     const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&q2);
     double s = 0.0;
 #pragma unroll
@@ -275,7 +276,7 @@ __device__ unsigned long long exact_score(const SparseAttentionParams& p, const 
 // computed scores near the cut do not settle it do the warps work together: the keys there are
 // replaced by the largest or the smallest one, by exact score (`index` and `score` are scratch).
 template <int GROUP, int KEEP>
-__device__ uint32_t cut_blocks(const SparseAttentionParams& p, const int* pages, int row, int h, int nb, int need,
+__device__ uint32_t cut_blocks(const SparseAttentionParams& p, const int* pages, int token, int h, int nb, int need,
                                float worst, uint32_t* keys, uint32_t* index, unsigned long long* score,
                                int* n_border) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -348,7 +349,7 @@ __device__ uint32_t cut_blocks(const SparseAttentionParams& p, const int* pages,
     if (keys[b] >= low && keys[b] <= high) index[atomicAdd(n_border, 1)] = static_cast<uint32_t>(b);
   __syncthreads();
   for (int i = warp; i < border; i += kSparseWarps) {
-    const unsigned long long s = exact_score<GROUP>(p, pages, row, h, static_cast<int>(index[i]));
+    const unsigned long long s = exact_score<GROUP>(p, pages, token, h, static_cast<int>(index[i]));
     if (lane == 0) score[i] = s;
   }
   __syncthreads();
@@ -384,7 +385,11 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
   const int h = blockIdx.y, row = blockIdx.z;
-  int len = p.seqused_k[row];
+  int len = p.seqused_k[row], token = row;
+  if (p.cu_seq_q != nullptr) {
+    token = p.cu_seq_q[row];
+    if (p.cu_seq_q[row + 1] - token != 1) return;  // the whole cluster
+  }
   for (int i = tid; i < p.width; i += kSparseThreads) pages[i] = p.block_table[static_cast<int64_t>(row) * p.width + i];
   if (len > p.width * p.page_size) {  // more keys than the table has pages for
     if (tid == 0 && rank == 0) raise_status(kStatusBadPage);
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
     const int last = nb - p.recent, groups = (nb + 7) / 8;
     const int b0 = 8 * (groups * rank / ranks), b1 = min(nb, 8 * (groups * (rank + 1) / ranks));
     for (int b = nb + tid; b < (nb + 127) / 128 * 128; b += kSparseThreads) keys[b] = 0u;
-    float worst = score_blocks<GROUP>(p, pages, row, h, b0, b1, last, keys, ranks);
+    float worst = score_blocks<GROUP>(p, pages, token, h, b0, b1, last, keys, ranks);
     worst = warp_max(worst);
     if (lane < ranks) {  // non-negative floats compare as their bits do
       uint32_t a;
@@ -420,8 +425,8 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
     if (ranks > 1) cluster_sync();
     else __syncthreads();
     const float size = __uint_as_float(sh.worst);
-    above = nb <= 640 ? cut_blocks<GROUP, 5>(p, pages, row, h, nb, need, size, keys, index, score, &sh.n_border)
-                      : cut_blocks<GROUP, 0>(p, pages, row, h, nb, need, size, keys, index, score, &sh.n_border);
+    above = nb <= 640 ? cut_blocks<GROUP, 5>(p, pages, token, h, nb, need, size, keys, index, score, &sh.n_border)
+                      : cut_blocks<GROUP, 0>(p, pages, token, h, nb, need, size, keys, index, score, &sh.n_border);
   }
   // Ascending list: four blocks per thread at a time, places by a scan over the CTA.
   int n_sel = 0;
@@ -503,7 +508,7 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
     DecodeUnit u{};
     u.h = h;
     u.row = row;
-    u.q0 = row;
+    u.q0 = token;
     u.count = 1;
     u.end = u.ke = len;
     u.qrows = GROUP;
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
         den += w * l[r];
       }
     }
-    p.out[(static_cast<int64_t>(row) * p.heads + h * GROUP + g) * 128 + d] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+    p.out[(static_cast<int64_t>(token) * p.heads + h * GROUP + g) * 128 + d] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
   }
   if (ranks > 1) cluster_sync();  // the parts stay until every CTA has read them
 }

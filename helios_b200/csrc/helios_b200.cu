@@ -892,8 +892,8 @@ int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_pages, i
 
 int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* value_pool, const void* bounds,
                               int64_t num_pages, int32_t page_size, const int32_t* block_table, int32_t width,
-                              const int32_t* seqused_k, int32_t num_rows, int32_t heads, int32_t kv_heads,
-                              int32_t head_dim, int32_t top_blocks, int32_t sink_blocks, int32_t recent_blocks,
+                              const int32_t* seqused_k, const int32_t* cu_seq_q, int32_t num_rows, int32_t heads,
+                              int32_t kv_heads, int32_t head_dim, int32_t top_blocks, int32_t sink_blocks, int32_t recent_blocks,
                               float scale, int32_t* selected, void* out, cudaStream_t stream) {
   if (head_dim != 128) return fail(HB_ERR_UNSUPPORTED, "sparse attention supports head_dim 128, got %d", head_dim);
   if (heads < 1 || kv_heads < 1 || heads % kv_heads) return fail(HB_ERR_INVALID, "bad head counts");
@@ -925,7 +925,7 @@ int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* v
     return rc;
   const int per_page = page_size / hb::kBlockKeys;
   hb::SparseAttentionParams p{static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out),
-                              static_cast<const __nv_bfloat16*>(bounds), block_table, seqused_k, selected, width,
+                              static_cast<const __nv_bfloat16*>(bounds), block_table, seqused_k, cu_seq_q, selected, width,
                               static_cast<int32_t>(num_pages), page_size, heads, kv_heads, per_page,
                               per_page > 1 ? static_cast<uint32_t>(((1ull << 32) + per_page - 1) / per_page) : 0u,
                               top_blocks, sink_blocks, recent_blocks, scale * 1.4426950408889634f};

@@ -2,6 +2,7 @@
 //
 // Restates Decoder._sample (src/helios/runtime/qwen3/decode.py:457-473) and its
 // batched use (src/helios/runtime/engine.py:470-492) without a sort:
+//   * a row without a logit above -inf: -1, no token;
 //   * temperature 0: argmax, first index among equal maxima;
 //   * otherwise p_i ~ exp(l_i / T - max / T). With top_p < 1, token i survives when
 //     the mass of the tokens ranked before it (descending probability, ties by
@@ -511,6 +512,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p) 
     }
   }
   const float gmax = block_reduce(mx, [](float a, float b) { return fmaxf(a, b); }, fred);
+  if (gmax == -INFINITY) {  // nothing to choose: a mask left no token (or every logit is NaN)
+    if (tid == 0) p.out[row] = -1;
+    return;
+  }
   if (mx != gmax) arg = INT_MAX;
   const int garg = block_reduce(arg, [](int a, int b) { return min(a, b); }, ired);
   if (greedy) {

@@ -33,7 +33,9 @@ import torch
 from helios_b200 import ops
 from helios_b200.config import Sampling
 from helios_b200.model import Qwen3Model
-from helios_b200.paged_cache import KVPagePool, PackedBatchCache, PagedBatchCache, PagedKVCache
+from helios_b200.controls import LogitControls, TokenHistory, control_rows
+from helios_b200.paged_cache import (KVPagePool, PackedBatchCache, PagedBatchCache, PagedKVCache,
+                                     SparseAttention)
 
 
 @dataclass
@@ -85,6 +87,7 @@ class Decoder:
         self.page_pool: KVPagePool | None = None
         self._paged_decode_batch: PagedBatchCache | None = None
         self._packed_batch: PackedBatchCache | None = None
+        self.sparse_attention: SparseAttention | None = None
 
     @property
     def device(self) -> torch.device:
@@ -265,6 +268,7 @@ class Decoder:
                 batch = self._paged_decode_batch = PagedBatchCache(caches)
             batch.caches = tuple(caches)
             batch.batch_size = len(caches)
+            self._set_sparse(batch)
             try:
                 if on_device:
                     tokens = token_ids.to(torch.long).unsqueeze(1)
@@ -277,6 +281,13 @@ class Decoder:
                 return self.model(tokens, cache=batch, cache_slots=slots)[:, -1, :]
             finally:
                 batch.caches = ()
+
+    def _set_sparse(self, batch: PagedBatchCache) -> None:
+        """``sparse_attention`` for a tick's rows with one token (no counterpart in the reference, whose
+        attention is dense): a ``SparseAttention``, or None for dense attention."""
+        batch.sparse = self.sparse_attention
+        if batch.sparse is not None and batch.pool.bounds is None:
+            batch.pool.enable_key_bounds()
 
     def packed_caches(self, caches: list[PagedKVCache], chunks: list[list[int]], *,
                       logit_counts: list[int] | None = None) -> torch.Tensor:
@@ -301,6 +312,7 @@ class Decoder:
             if batch is None or batch.pool is not caches[0].pool:
                 batch = self._packed_batch = PackedBatchCache(caches)
             batch.caches, batch.batch_size = tuple(caches), len(caches)
+            self._set_sparse(batch)
             try:
                 tokens = batch.metadata("token_ids", [t for chunk in chunks for t in chunk], torch.long).unsqueeze(0)
                 batch.prepare_packed([len(chunk) for chunk in chunks], logit_counts)
@@ -318,8 +330,12 @@ class Decoder:
 
 
 def sample_rows(logits: torch.Tensor, samplings: Sequence[Sampling], *, uniforms: torch.Tensor | None = None,
-                generator: torch.Generator | None = None) -> torch.Tensor:
-    """One token id per logit row with per-row temperature / top-p (kernel d)."""
+                generator: torch.Generator | None = None,
+                controls: Sequence[LogitControls | None] | None = None,
+                history: TokenHistory | None = None) -> torch.Tensor:
+    """One token id per logit row with per-row temperature / top-p (kernel d). ``controls`` puts each
+    row's penalties, biases and mask on its logits first (``controls.control_rows``; ``logits`` itself
+    stays as it is). A row in which they leave no token gives -1."""
     rows = logits.shape[0]
     if len(samplings) != rows:
         raise ValueError("Each logit row needs its sampling settings.")
@@ -336,6 +352,8 @@ def sample_rows(logits: torch.Tensor, samplings: Sequence[Sampling], *, uniforms
         uniforms = uniforms.to(device=device, dtype=torch.float32)
     if logits.dtype != torch.bfloat16:
         logits = logits.to(torch.bfloat16)
+    if controls is not None:
+        logits = control_rows(logits, controls, history)
     return ops.sample(logits, settings[:, 0].contiguous(), settings[:, 1].contiguous(), uniforms.contiguous())
 
 

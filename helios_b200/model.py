@@ -38,6 +38,7 @@ from torch import nn
 from helios_b200 import ops
 from helios_b200.config import Qwen3Config
 from helios_b200.paged_cache import PackedBatchCache, PagedBatchCache
+from helios_b200.w4 import W4Linear, quantize_w4
 
 
 class RMSNorm(nn.Module):
@@ -103,6 +104,13 @@ class _Fused:
         return self.weight
 
 
+def _drop(*linears: nn.Linear) -> None:
+    """Free weights that a 4-bit copy has replaced. The parameters stay, empty, so that loading a
+    full-precision state dict into the model fails by their shapes."""
+    for linear in linears:
+        linear.weight = nn.Parameter(linear.weight.new_empty(0), requires_grad=False)
+
+
 class FeedForward(nn.Module):
     def __init__(self, config: Qwen3Config) -> None:
         super().__init__()
@@ -110,6 +118,14 @@ class FeedForward(nn.Module):
         self.up = nn.Linear(config.hidden_size, config.hidden_dim, bias=False, dtype=config.dtype)
         self.down = nn.Linear(config.hidden_dim, config.hidden_size, bias=False, dtype=config.dtype)
         self._gate_up = _Fused(self.gate, self.up)
+        self.w4_gate_up: W4Linear | None = None  # set by quantize
+        self.w4_down: W4Linear | None = None
+
+    def quantize(self, group_size: int, symmetric: bool) -> None:
+        self.w4_gate_up = W4Linear(quantize_w4(self._gate_up.get(), group_size, symmetric=symmetric))
+        self.w4_down = W4Linear(quantize_w4(self.down.weight, group_size, symmetric=symmetric))
+        self._gate_up = None
+        _drop(self.gate, self.up, self.down)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """``x [T, hidden]`` -> ``[T, hidden]``: gate|up projection + SwiGLU, then the down GEMM.
@@ -117,6 +133,10 @@ class FeedForward(nn.Module):
         with SwiGLU in its epilogue; fewer rows (mostly padding in its 128-row tiles) take
         cuBLAS and the SwiGLU kernel. Both keep the reference's rounding points."""
         inter = self.gate.out_features
+        if self.w4_gate_up is not None:
+            gate_up = self.w4_gate_up(x)
+            act = torch.empty((x.shape[0], inter), dtype=x.dtype, device=x.device)
+            return self.w4_down(ops.swiglu(gate_up, act))
         if x.shape[0] >= FUSED_GATE_UP_MIN_ROWS and x.shape[1] % 64 == 0 and inter % 128 == 0:
             act = ops.gemm_swiglu(x.contiguous(), self._gate_up.get())
         else:
@@ -142,15 +162,24 @@ class GroupedQueryAttention(nn.Module):
         self.q_norm = RMSNorm(config.head_dim, config.rms_norm_eps)
         self.k_norm = RMSNorm(config.head_dim, config.rms_norm_eps)
         self._qkv = _Fused(self.query, self.key, self.value)
+        self.w4_qkv: W4Linear | None = None  # set by quantize
+        self.w4_output: W4Linear | None = None
+
+    def quantize(self, group_size: int, symmetric: bool) -> None:
+        self.w4_qkv = W4Linear(quantize_w4(self._qkv.get(), group_size, symmetric=symmetric))
+        self.w4_output = W4Linear(quantize_w4(self.output.weight, group_size, symmetric=symmetric))
+        self._qkv = None
+        _drop(self.query, self.key, self.value, self.output)
 
     def forward(self, x: torch.Tensor, cache: PagedBatchCache, layer_index: int, cos: torch.Tensor,
                 sin: torch.Tensor) -> torch.Tensor:
         """``x [T, hidden]`` (already input-normed) -> attention block output ``[T, hidden]``:
         one cuBLAS GEMM for q|k|v, kernel (b) (norm, RoPE, KV append), kernel (c), o-proj."""
-        qkv = F.linear(x, self._qkv.get())
+        qkv = F.linear(x, self._qkv.get()) if self.w4_qkv is None else self.w4_qkv(x)
         context = cache.attend_fused(layer_index, qkv, self.q_norm.scale, self.k_norm.scale, self.q_norm.eps,
                                      cos, sin)
-        return F.linear(context.view(x.shape[0], -1), self.output.weight)
+        context = context.view(x.shape[0], -1)
+        return F.linear(context, self.output.weight) if self.w4_output is None else self.w4_output(context)
 
 
 class TransformerBlock(nn.Module):
@@ -196,6 +225,20 @@ class Qwen3Model(nn.Module):
         if missing or unexpected:
             raise ValueError(f"state dict does not match the model: missing {missing}, unexpected {unexpected}")
         return model.eval()
+
+    def quantize_weights(self, group_size: int = 128, *, symmetric: bool = True) -> None:
+        """Hold every block's projections in 4 bits from here on (``helios_b200.w4.quantize_w4``: groups
+        of 32, 64 or 128 along the input dimension); the bf16 weights are freed. Embedding, lm_head and
+        norms stay as they are. Ticks then read a quarter of the weight bytes: the Qwen3-4B shape's
+        blocks shrink from 7.3 to 1.9 GB. There is no counterpart in the reference."""
+        for block in self.blocks:
+            if block.feed_forward.w4_gate_up is not None:
+                raise RuntimeError("The model's weights are already quantized.")
+        for block in self.blocks:
+            block.attention.quantize(group_size, symmetric)
+            block.feed_forward.quantize(group_size, symmetric)
+        if self._graphs is not None:  # captured ticks run the freed weights
+            self.enable_cuda_graphs(self._graphs.max_graphs)
 
     def enable_cuda_graphs(self, max_graphs: int = 4) -> None:
         """Replay the device half of packed ticks from CUDA graphs (see helios_b200.graphs).

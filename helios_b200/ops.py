@@ -297,7 +297,8 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
     return out
 
 
-BLOCK_KEYS = 64  # keys per block of the sparse attention
+BLOCK_KEYS = 64        # keys per block of the sparse attention
+MAX_TOP_BLOCKS = 1024  # blocks it attends to at most
 
 
 def _check_bounds(key_pool: torch.Tensor, bounds: torch.Tensor) -> None:
@@ -345,7 +346,8 @@ def key_block_bounds(key_pool: torch.Tensor, bounds: torch.Tensor, block_table: 
     return bounds
 
 
-def _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, out, selected, top_blocks) -> None:
+def _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, cu_seq_q, out, selected,
+                   top_blocks) -> None:
     _need(q, BF16, "q")
     _need(value_pool, BF16, "value_pool")
     _check_bounds(key_pool, bounds)
@@ -353,31 +355,41 @@ def _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, out,
     _need(seqused_k, I32, "seqused_k")
     if q.dim() != 3 or value_pool.shape != key_pool.shape or q.shape[2] != key_pool.shape[3]:
         raise ValueError("q must be [rows, heads, head_dim], and both pools must match each other and its head_dim")
-    if block_table.dim() != 2 or block_table.shape[0] != q.shape[0] or seqused_k.numel() != q.shape[0]:
-        raise ValueError("block_table and seqused_k need one row per query row")
+    if block_table.dim() != 2 or seqused_k.numel() != block_table.shape[0]:
+        raise ValueError("block_table and seqused_k need one row per sequence")
+    if cu_seq_q is not None:
+        _need(cu_seq_q, I32, "cu_seq_q")
+        if cu_seq_q.numel() != block_table.shape[0] + 1:
+            raise ValueError("cu_seq_q needs rows + 1 entries")
+    elif block_table.shape[0] != q.shape[0]:
+        raise ValueError("without cu_seq_q, q needs one token per row")
     if out is not None:
         _need(out, BF16, "out")
         if out.shape != q.shape:
             raise ValueError("out must have the shape of q")
     if selected is not None:
         _need(selected, I32, "selected")
-        if selected.shape != (q.shape[0], key_pool.shape[2], top_blocks):
+        if selected.shape != (block_table.shape[0], key_pool.shape[2], top_blocks):
             raise ValueError("selected must be [rows, kv_heads, top_blocks]")
     _together(q.device, key_pool=key_pool, value_pool=value_pool, bounds=bounds, block_table=block_table,
-              seqused_k=seqused_k, out=out, selected=selected)
-    raise ValueError("sparse_paged_attention arguments do not fit together")
+              seqused_k=seqused_k, cu_seq_q=cu_seq_q, out=out, selected=selected)
+    raise ValueError("sparse_paged_attention with cu_seq_q needs out")
 
 
 def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, bounds: torch.Tensor,
                            block_table: torch.Tensor, seqused_k: torch.Tensor, out: torch.Tensor | None = None, *,
                            top_blocks: int, sink_blocks: int = 1, recent_blocks: int = 2,
-                           scale: float | None = None, selected: torch.Tensor | None = None) -> torch.Tensor:
+                           scale: float | None = None, selected: torch.Tensor | None = None,
+                           cu_seq_q: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one query token per row, ``q [rows, H, d]``, over the ``top_blocks`` 64-key blocks
     that the ``bounds`` of key_block_bounds select for it and each KV head, the row's first
     ``sink_blocks`` and last ``recent_blocks`` blocks always among them (hb_sparse_paged_attention).
     ``selected`` (int32 ``[rows, Hkv, top_blocks]``) gets the blocks in ascending order, then -1.
-    Returns ``out [rows, H, d]``, or a new tensor; a row without keys gives zeros."""
+    Returns ``out [rows, H, d]``, or a new tensor; a row without keys gives zeros. With ``cu_seq_q``
+    (int32 ``[rows + 1]``) ``q`` and ``out`` are ``[tokens, H, d]``, row r's token is ``cu_seq_q[r]``, and
+    rows with other than one token are left as ``out`` has them (it has to be given then)."""
     dev = q.device
+    refuse = (q, key_pool, value_pool, bounds, block_table, seqused_k, cu_seq_q, out, selected, top_blocks)
     if not (q.is_cuda and q.dtype is BF16 and key_pool.dtype is BF16 and value_pool.dtype is BF16
             and bounds.dtype is BF16 and block_table.dtype is I32 and seqused_k.dtype is I32
             and key_pool.device == dev and value_pool.device == dev and bounds.device == dev
@@ -385,23 +397,26 @@ def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
             and key_pool.is_contiguous() and value_pool.is_contiguous() and bounds.is_contiguous()
             and block_table.is_contiguous() and seqused_k.is_contiguous() and q.dim() == 3 and key_pool.dim() == 4
             and block_table.dim() == 2):
-        _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, out, selected, top_blocks)
-    rows, heads, dim = q.shape
+        _refuse_sparse(*refuse)
+    tokens, heads, dim = q.shape
     pool_shape = key_pool.shape
     pages, page, kv_heads, pool_dim = pool_shape
-    table_rows, width = block_table.shape
-    if not (value_pool.shape == pool_shape and dim == pool_dim and table_rows == rows and seqused_k.numel() == rows
+    rows, width = block_table.shape
+    if not (value_pool.shape == pool_shape and dim == pool_dim and seqused_k.numel() == rows
+            and (tokens == rows if cu_seq_q is None else
+                 cu_seq_q.dtype is I32 and cu_seq_q.device == dev and cu_seq_q.is_contiguous()
+                 and cu_seq_q.numel() == rows + 1 and out is not None)
             and bounds.shape == (pages, kv_heads, page // BLOCK_KEYS, 2, dim)
             and (out is None or (out.dtype is BF16 and out.device == dev and out.is_contiguous()
                                  and out.shape == q.shape))
             and (selected is None or (selected.dtype is I32 and selected.device == dev and selected.is_contiguous()
                                       and selected.shape == (rows, kv_heads, top_blocks)))):
-        _refuse_sparse(q, key_pool, value_pool, bounds, block_table, seqused_k, out, selected, top_blocks)
+        _refuse_sparse(*refuse)
     if out is None:
         out = torch.empty_like(q)
     _call(lib().hb_sparse_paged_attention, "hb_sparse_paged_attention", dev, q.data_ptr(), key_pool.data_ptr(),
           value_pool.data_ptr(), bounds.data_ptr(), pages, page, block_table.data_ptr(), width, seqused_k.data_ptr(),
-          rows, heads, kv_heads, dim, top_blocks, sink_blocks, recent_blocks, dim ** -0.5 if scale is None else scale,
+          None if cu_seq_q is None else cu_seq_q.data_ptr(), rows, heads, kv_heads, dim, top_blocks, sink_blocks, recent_blocks, dim ** -0.5 if scale is None else scale,
           None if selected is None else selected.data_ptr(), out.data_ptr())
     return out
 

@@ -58,6 +58,23 @@ class KVPage:
 
 
 @dataclass(frozen=True)
+class SparseAttention:
+    """Which keys a row with one query token attends to: ``top_blocks`` blocks of 64 keys per KV head,
+    the first ``sink_blocks`` and the last ``recent_blocks`` always among them, the others chosen by
+    the bounds of their keys (``ops.sparse_paged_attention``). Rows of at most ``top_blocks`` blocks
+    attend to all of their keys."""
+    top_blocks: int = 32
+    sink_blocks: int = 1
+    recent_blocks: int = 2
+
+    def __post_init__(self) -> None:
+        if self.sink_blocks < 0 or self.recent_blocks < 1 or not (
+                self.sink_blocks + self.recent_blocks <= self.top_blocks <= ops.MAX_TOP_BLOCKS):
+            raise ValueError("top_blocks must hold sink_blocks >= 0 and recent_blocks >= 1 and be at most "
+                             f"{ops.MAX_TOP_BLOCKS}")
+
+
+@dataclass(frozen=True)
 class PagedKVBlockSnapshot:
     length: int
     pages: tuple[KVPage, ...]
@@ -84,6 +101,9 @@ class KVPagePool:
             dtype=config.dtype, device=self.device)
         self.keys = tuple(self.storage[layer, 0] for layer in range(config.n_layers))
         self.values = tuple(self.storage[layer, 1] for layer in range(config.n_layers))
+        # Per layer [pages, Hkv, page / 64, 2, d], minima then maxima of the keys of 64-key blocks; None
+        # until enable_key_bounds.
+        self.bounds: torch.Tensor | None = None
         self._free = list(range(num_pages - 1, -1, -1))
         self.arena_width = _pages_for(config.context_length, page_size)
         self._arena = torch.zeros((0, self.arena_width), dtype=torch.int32, device=self.device)
@@ -110,6 +130,21 @@ class KVPagePool:
 
     def _release(self, index: int) -> None:
         self._free.append(index)
+
+    def enable_key_bounds(self) -> None:
+        """Keep the bounds that sparse attention selects key blocks by: 1/64 of the pool's size. Keys
+        appended before count too. From here on every tick brings the bounds of the blocks it writes
+        up to date, for every cache of this pool."""
+        if self.bounds is not None:
+            return
+        config, blocks = self.config, self.page_size // ops.BLOCK_KEYS
+        bounds = torch.empty((config.n_layers, self.num_pages, config.n_kv_heads, blocks, 2, config.head_dim),
+                             dtype=config.dtype, device=self.device)
+        for layer, keys in enumerate(self.keys):
+            parts = keys.view(self.num_pages, blocks, ops.BLOCK_KEYS, config.n_kv_heads, config.head_dim)
+            bounds[layer, :, :, :, 0].copy_(parts.amin(2).transpose(1, 2))
+            bounds[layer, :, :, :, 1].copy_(parts.amax(2).transpose(1, 2))
+        self.bounds = bounds
 
     # ---- device page arena (one slot per live request cache)
     @property
@@ -141,6 +176,8 @@ class KVPagePool:
         pairs = torch.tensor([list(src), list(dst)], dtype=torch.int32).to(self.device)
         flat = self.storage.view(2 * self.config.n_layers, self.num_pages, *self.storage.shape[3:])
         ops.page_copy(flat, pairs[0], pairs[1])
+        if self.bounds is not None:
+            ops.page_copy(self.bounds, pairs[0], pairs[1])
 
 
 class PagedKVCache:
@@ -300,6 +337,7 @@ class PagedBatchCache:
         self.attention_counts: torch.Tensor | None = None
         self.launch_decode_items = self.launch_prefill_items = self.launch_partial_records = 0
         self.launch_prefix_items = self.num_prefix_items = 0
+        self.sparse: SparseAttention | None = None  # single-token rows attend to selected key blocks
 
     @property
     def length(self) -> int:
@@ -582,9 +620,30 @@ class PagedBatchCache:
         ops.qk_norm_rope_append(None, k, v, q_scale=None, k_scale=None, eps=0.0, cos=None, sin=None, positions=None,
                                 write_slots=self.write_slots, q_out=None, key_pool=pool.keys[layer],
                                 value_pool=pool.values[layer])
-        q = q.contiguous()
+        return self._attention(layer, q.contiguous())
+
+    def _attention(self, layer: int, q: torch.Tensor) -> torch.Tensor:
+        """Attention of the tick's tokens ``q [T, H, d]`` once their keys and values are in the pool. With
+        ``sparse`` set, rows with one token attend to selected blocks, whatever else the tick holds; a
+        tick of such rows alone skips the dense kernels, in others their dense results are replaced."""
+        pool = self.pool
+        keys, values = pool.keys[layer], pool.values[layer]
+        if pool.bounds is not None:
+            ops.key_block_bounds(keys, pool.bounds[layer], self.block_table, self.cu_seq_q, self.seqused_k,
+                                 self.token_row)
         out = torch.empty_like(q)
-        return ops.paged_attention(q, pool.keys[layer], pool.values[layer], self, out)
+        sparse = self.sparse
+        single = self.total_tokens == self.batch_size
+        if sparse is None or not single:
+            ops.paged_attention(q, keys, values, self, out)
+        if sparse is not None:
+            if pool.bounds is None:
+                raise RuntimeError("Sparse attention needs the pool's key bounds (KVPagePool.enable_key_bounds).")
+            ops.sparse_paged_attention(q, keys, values, pool.bounds[layer], self.block_table, self.seqused_k, out,
+                                       top_blocks=sparse.top_blocks, sink_blocks=sparse.sink_blocks,
+                                       recent_blocks=sparse.recent_blocks,
+                                       cu_seq_q=None if single else self.cu_seq_q)
+        return out
 
     def attend_fused(self, layer: int, qkv: torch.Tensor, q_scale: torch.Tensor, k_scale: torch.Tensor, eps: float,
                      cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
@@ -603,8 +662,7 @@ class PagedBatchCache:
         ops.qk_norm_rope_append(q, k, v, q_scale=q_scale, k_scale=k_scale, eps=eps, cos=cos, sin=sin,
                                 positions=self.token_positions, write_slots=self.write_slots, q_out=q_rot,
                                 key_pool=pool.keys[layer], value_pool=pool.values[layer])
-        out = torch.empty_like(q_rot)
-        return ops.paged_attention(q_rot, pool.keys[layer], pool.values[layer], self, out)
+        return self._attention(layer, q_rot)
 
 
 def _validate_attention_inputs(cache: PagedBatchCache, layer: int, queries, keys, values) -> int:

@@ -17,6 +17,9 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch import nn
+
+from helios_b200 import ops
 
 GROUPS = (32, 64, 128)
 NIBBLE_SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)  # bit position of k = 8c + i in word c
@@ -87,3 +90,20 @@ def dequantize_w4(weight: W4Weight, dtype: torch.dtype = torch.float32) -> torch
     codes = unpack_w4(weight.packed).view(n, groups, -1).to(torch.float64)
     zeros = 8.0 if weight.zeros is None else (weight.zeros & 15).t().unsqueeze(-1).to(torch.float64)
     return ((codes - zeros) * weight.scales.t().unsqueeze(-1).to(torch.float64)).reshape(n, -1).to(dtype)
+
+
+class W4Linear(nn.Module):
+    """A bias-free Linear whose weight is held in 4 bits (``ops.linear_w4``). The tensors are
+    buffers, so they move with the model; they are not part of its state dict."""
+
+    def __init__(self, weight: W4Weight) -> None:
+        super().__init__()
+        for name in W4Weight._fields:
+            self.register_buffer(name, getattr(weight, name), persistent=False)
+
+    @property
+    def weight(self) -> W4Weight:
+        return W4Weight(self.packed, self.scales, self.zeros)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return ops.linear_w4(x, self.packed, self.scales, self.zeros)

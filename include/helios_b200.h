@@ -278,15 +278,17 @@ HB_API int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_p
  * takes the row's first sink_blocks and last recent_blocks blocks and, of the others, those with
  * the largest max over the head's query group of sum_d max(q_d lo_d, q_d hi_d), top_blocks in
  * all; equal scores go to the lower block, NaN ranks first. Scores are compared exactly.
- * q and out bf16 [num_rows][heads][head_dim]; selected int32 [num_rows][kv_heads][top_blocks]
+ * q and out bf16 [tokens][heads][head_dim]: row r's token is cu_seq_q[r], and rows whose
+ * cu_seq_q range holds other than one token are left as they are (out and selected); with
+ * cu_seq_q null row r's token is r. selected int32 [num_rows][kv_heads][top_blocks]
  * (may be null) gets the blocks in ascending order, then -1. Needs head_dim 128, 1, 2, 4 or 8
  * query heads per KV head, top_blocks <= 1024 and width * page_size <= 393,216 tokens.
  */
 HB_API int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* value_pool, const void* bounds,
                                      int64_t num_pages, int32_t page_size, const int32_t* block_table, int32_t width,
-                                     const int32_t* seqused_k, int32_t num_rows, int32_t heads, int32_t kv_heads,
-                                     int32_t head_dim, int32_t top_blocks, int32_t sink_blocks,
-                                     int32_t recent_blocks, float scale, int32_t* selected, void* out,
+                                     const int32_t* seqused_k, const int32_t* cu_seq_q, int32_t num_rows,
+                                     int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t top_blocks,
+                                     int32_t sink_blocks, int32_t recent_blocks, float scale, int32_t* selected, void* out,
                                      cudaStream_t stream);
 
 /*
@@ -366,7 +368,8 @@ HB_API int hb_page_copy(void* pool_base, int64_t tensor_stride_bytes, int32_t te
  * and the batched sampling in Engine._execute_batch (src/helios/runtime/engine.py:470-492).
  * temperature 0 -> argmax (first index); otherwise temperature softmax with the
  * reference's top-p keep rule, drawn by inverse CDF over kept tokens in index order
- * with the caller's uniforms[rows] in [0, 1). logits bf16 [rows][row_stride].
+ * with the caller's uniforms[rows] in [0, 1). A row without a logit above -inf (a mask that left
+ * nothing) gives -1. logits bf16 [rows][row_stride].
  */
 HB_API int hb_sample(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab, const float* temperature,
                      const float* top_p, const float* uniforms, int64_t* out_ids, cudaStream_t stream);

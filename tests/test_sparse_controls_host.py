@@ -19,7 +19,7 @@ def lib():
 
 
 def sparse(lib, rows=1, heads=8, kv_heads=2, dim=128, page=256, width=4, top=8, sink=1, recent=2, q=P, pages=10):
-    return lib.hb_sparse_paged_attention(q, P, P, P, pages, page, P, width, P, rows, heads, kv_heads, dim, top, sink,
+    return lib.hb_sparse_paged_attention(q, P, P, P, pages, page, P, width, P, None, rows, heads, kv_heads, dim, top, sink,
                                          recent, ctypes.c_float(0.1), None, P, None)
 
 
