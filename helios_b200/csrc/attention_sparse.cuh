@@ -37,56 +37,95 @@ struct BlockBoundsParams {
   int32_t rows, tokens, width, num_pages, page_size, kv_heads;
 };
 
-constexpr int kBoundsThreads = 256;
+constexpr int kBoundsThreads = 512;
 
-// One CTA per token of the tick; the CTA of the first token that a row has in a block (in this
-// tick) computes the block's bounds anew from the pool, over the keys the row has there by now.
-// Nothing is carried over from earlier bounds, so truncated and rewritten keys leave no trace.
-// A warp takes a KV head's keys: 8 bytes per lane, a 256-byte row per load.
-__global__ void __launch_bounds__(kBoundsThreads) key_block_bounds_kernel(BlockBoundsParams p) {
-  const int token = blockIdx.x;
-  const int row = p.token_row[token];
-  if (row < 0 || row >= p.rows) {
-    if (threadIdx.x == 0) raise_status(kStatusBadRow);
-    return;
-  }
-  const int q0 = p.cu_seq_q[row], count = p.cu_seq_q[row + 1] - q0, end = p.seqused_k[row];
-  const int pos = end - count + (token - q0);
-  if (pos < 0 || pos >= end) return;
-  if (token != q0 && pos % kBlockKeys != 0) return;
-  const int first = pos - pos % kBlockKeys, n = min(kBlockKeys, end - first);
-  const int pidx = first / p.page_size;
-  const int page = pidx < p.width ? p.block_table[static_cast<int64_t>(row) * p.width + pidx] : -1;
-  if (page < 0 || page >= p.num_pages) {
-    if (threadIdx.x == 0) raise_status(kStatusBadPage);
-    return;
-  }
+// The bounds of the n keys from key `at` of a page, by the whole CTA.
+__device__ __forceinline__ void block_bounds_of(const BlockBoundsParams& p, int page, int at, int n, uint4 (*other)[2][16]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int at = first % p.page_size;
-  for (int h = warp; h < p.kv_heads; h += kBoundsThreads / 32) {
-    const __nv_bfloat16* src =
-        p.keys + ((static_cast<int64_t>(page) * p.page_size + at) * p.kv_heads + h) * 128 + 4 * lane;
-    const int64_t step = static_cast<int64_t>(p.kv_heads) * 128;
-    __nv_bfloat162 lo[2], hi[2];
-    *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(src);
-    hi[0] = lo[0];
-    hi[1] = lo[1];
-#pragma unroll 16
-    for (int i = 1; i < kBlockKeys; ++i) {
-      if (i < n) {
-        __nv_bfloat162 v[2];
-        *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(src + i * step);
-        lo[0] = __hmin2_nan(lo[0], v[0]);
-        lo[1] = __hmin2_nan(lo[1], v[1]);
-        hi[0] = __hmax2_nan(hi[0], v[0]);
-        hi[1] = __hmax2_nan(hi[1], v[1]);
+  const int pair = warp >> 1, part = warp & 1, half = lane >> 4, col = lane & 15;  // 16 bytes per lane
+  const int blocks = p.page_size / kBlockKeys;
+  const int64_t step = static_cast<int64_t>(p.kv_heads) * 128;
+  for (int h0 = 0; h0 < p.kv_heads; h0 += kBoundsThreads / 64) {  // the same for the whole CTA
+    const int h = h0 + pair;
+    __nv_bfloat162 lo[4], hi[4];
+    if (h < p.kv_heads) {
+      const __nv_bfloat16* src =
+          p.keys + ((static_cast<int64_t>(page) * p.page_size + at) * p.kv_heads + h) * 128 + 8 * col;
+      uint4 v[kBlockKeys / 4];
+#pragma unroll
+      for (int i = 0; i < kBlockKeys / 4; ++i) {
+        const int key = min(32 * part + 2 * i + half, n - 1);
+        v[i] = *reinterpret_cast<const uint4*>(src + key * step);
+      }
+      *reinterpret_cast<uint4*>(lo) = v[0];
+      *reinterpret_cast<uint4*>(hi) = v[0];
+#pragma unroll
+      for (int i = 1; i < kBlockKeys / 4; ++i) {
+        const __nv_bfloat162* k = reinterpret_cast<const __nv_bfloat162*>(&v[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = __hmin2_nan(lo[e], k[e]);
+          hi[e] = __hmax2_nan(hi[e], k[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // the other half-warp's keys
+        lo[e] = __hmin2_nan(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], 16));
+        hi[e] = __hmax2_nan(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], 16));
+      }
+      if (part == 1 && half == 0) {
+        other[pair][0][col] = *reinterpret_cast<uint4*>(lo);
+        other[pair][1][col] = *reinterpret_cast<uint4*>(hi);
       }
     }
-    const int blocks = p.page_size / kBlockKeys;
-    __nv_bfloat16* dst =
-        p.bounds + ((static_cast<int64_t>(page) * p.kv_heads + h) * blocks + at / kBlockKeys) * 256 + 4 * lane;
-    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(lo);
-    *reinterpret_cast<uint2*>(dst + 128) = *reinterpret_cast<uint2*>(hi);
+    __syncthreads();
+    if (h < p.kv_heads && part == 0) {  // half-warp 0 writes the minima, 1 the maxima
+      const uint4 o = other[pair][half][col];
+      const __nv_bfloat162* k = reinterpret_cast<const __nv_bfloat162*>(&o);
+      __nv_bfloat162 r[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = half == 0 ? __hmin2_nan(lo[e], k[e]) : __hmax2_nan(hi[e], k[e]);
+      __nv_bfloat16* dst = p.bounds + ((static_cast<int64_t>(page) * p.kv_heads + h) * blocks + at / kBlockKeys) * 256;
+      *reinterpret_cast<uint4*>(dst + 128 * half + 8 * col) = *reinterpret_cast<uint4*>(r);
+    }
+    __syncthreads();  // `other` is written again
+  }
+}
+
+constexpr int kBoundsCtas = 293;  // two per SM, and a number that spreads every 64th token over them
+
+// The first token that a row has in a block (in this tick) stands for the block, and its bounds are
+// computed anew from the pool, over the keys the row has there by now. Nothing is carried over from
+// earlier bounds, so truncated and rewritten keys leave no trace. CTA b looks at tokens b, b + grid,
+// ..., a thread each, and then takes the blocks that it found one after the other: a decode tick has
+// a block per CTA, and a chunk's blocks, one in 64 tokens, spread evenly. (A CTA per token took 11
+// us for a 2048-token chunk and 80 us for 16,384.) What bounds it is latency: the row's description
+// is two reads deep, then the page, then the keys. Two warps share a KV head, a half-warp reads a
+// key's 256 bytes, and a warp's 32 keys are all asked for at once. Keys past the row's end repeat its
+// last one.
+__global__ void __launch_bounds__(kBoundsThreads) key_block_bounds_kernel(BlockBoundsParams p) {
+  __shared__ uint4 other[kBoundsThreads / 64][2][16];  // a head's second warp: minima, maxima
+  __shared__ int3 found[kBoundsThreads];               // page, first key in it, keys
+  __shared__ int n_found;
+  for (int64_t t0 = blockIdx.x; t0 < p.tokens; t0 += static_cast<int64_t>(kBoundsThreads) * gridDim.x) {
+    if (threadIdx.x == 0) n_found = 0;
+    __syncthreads();
+    const int64_t token = t0 + static_cast<int64_t>(threadIdx.x) * gridDim.x;
+    const int row = token < p.tokens ? p.token_row[token] : 0;
+    if (row < 0 || row >= p.rows) raise_status(kStatusBadRow);
+    else if (token < p.tokens) {
+      const int q0 = p.cu_seq_q[row], count = p.cu_seq_q[row + 1] - q0, end = p.seqused_k[row];
+      const int pos = end - count + static_cast<int>(token - q0);
+      if (pos >= 0 && pos < end && (token == q0 || pos % kBlockKeys == 0)) {
+        const int first = pos - pos % kBlockKeys, pidx = first / p.page_size;
+        const int page = pidx < p.width ? p.block_table[static_cast<int64_t>(row) * p.width + pidx] : -1;
+        if (page < 0 || page >= p.num_pages) raise_status(kStatusBadPage);
+        else found[atomicAdd(&n_found, 1)] = make_int3(page, first % p.page_size, min(kBlockKeys, end - first));
+      }
+    }
+    __syncthreads();
+    const int blocks = n_found;
+    for (int b = 0; b < blocks; ++b) block_bounds_of(p, found[b].x, found[b].y, found[b].z, other);
   }
 }
 

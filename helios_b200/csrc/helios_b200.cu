@@ -886,7 +886,7 @@ int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_pages, i
   hb::BlockBoundsParams p{static_cast<const __nv_bfloat16*>(key_pool), static_cast<__nv_bfloat16*>(bounds), block_table,
                           cu_seq_q, seqused_k, token_row, num_rows, total_tokens, width,
                           static_cast<int32_t>(num_pages), page_size, kv_heads};
-  hb::key_block_bounds_kernel<<<total_tokens, hb::kBoundsThreads, 0, stream>>>(p);
+  hb::key_block_bounds_kernel<<<std::min(total_tokens, hb::kBoundsCtas), hb::kBoundsThreads, 0, stream>>>(p);
   return check_launch("key_block_bounds_kernel");
 }
 
