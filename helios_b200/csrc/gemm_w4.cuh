@@ -9,9 +9,9 @@
 // one, at the cost of one fp32 FMA per output and group.
 //
 //   warp 0         TMA of the activations: per step of 128 k's two [NT tokens x 64 k] boxes
-//   warp 1         tensor memory; issues the MMAs, eight of K 16 per step
-//   warp 2         TMA of the packed weights: [128 rows x 256 k] boxes of 16 KB
-//   warp 3         scales and zero points into shared memory, eight groups at a time
+//   warps 1, 3     issue the MMAs, eight of K 16 per step, taking steps in turn; tensor memory
+//   warp 2         TMA of the packed weights: [128 rows x 256 k] boxes of 16 KB; scales and zero
+//                  points into shared memory, eight groups at a time
 //   warps 4..11    unpack: thread = weight row (TMEM lane), two warps per lane quadrant taking
 //                  steps in turn
 //   warps 12..19   scale and add: thread = weight row and half of the tokens; then the output
@@ -35,7 +35,8 @@ struct GemmW4Params {
   const __nv_bfloat16* scales;  // [k / G, n]
   const uint8_t* zeros;         // [k / G, n] or null
   __nv_bfloat16* out;           // [m, n]
-  int32_t m, n, k, tiles_m, tiles_n;  // token tiles, weight tiles
+  int32_t m, n, k, tiles_m;  // token tiles
+  int32_t tile0, tiles;      // of the tiles in order (token tiles fastest), the first and the number of this launch
 };
 
 constexpr int kW4gRows = 128;
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
   uint8_t* packed = smem;
   uint8_t* xs = smem + SP * kW4gPackedBytes;
-  __shared__ uint64_t full_p[SP], empty_p[SP], ready[S], done[S], full_s[kW4gScaleStages], empty_s[kW4gScaleStages], drain_bar;
+  __shared__ uint64_t full_p[SP], empty_p[SP], ready[S], done[S], full_s[kW4gScaleStages], empty_s[kW4gScaleStages], drain_bar[2];
   __shared__ __nv_bfloat16 scale_s[kW4gScaleStages][kW4gScaleGroups][kW4gRows];
   __shared__ uint8_t zero_s[kW4gScaleStages][kW4gScaleGroups][kW4gRows];
   __shared__ uint32_t tmem_base_s;
@@ -86,8 +87,8 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
-  const int tiles = p.tiles_m * p.tiles_n;
-  const int first_tile = static_cast<int>(blockIdx.x) / splits, tile_step = static_cast<int>(gridDim.x) / splits;
+  const int tiles = p.tile0 + p.tiles;  // their end
+  const int first_tile = p.tile0 + static_cast<int>(blockIdx.x) / splits, tile_step = static_cast<int>(gridDim.x) / splits;
   // This CTA's k's: whole units of 128, up to k's end.
   const int units = (p.k + 127) / 128;
   const int k0 = 128 * (units * rank / splits), k1 = min(p.k, 128 * (units * (rank + 1) / splits));
@@ -109,7 +110,8 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
       mbar_init(&full_s[s], 1);
       mbar_init(&empty_s[s], kW4gAddWarps + (p.zeros != nullptr ? kW4gUnpackWarps : 0));
     }
-    mbar_init(&drain_bar, 1);
+    mbar_init(&drain_bar[0], 1);
+    mbar_init(&drain_bar[1], 1);
     abort_flag = 0;
     fence_barrier_init();
   }
@@ -122,6 +124,7 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
   const uint32_t tmem_a = tmem + 256;
+  pdl_trigger();  // a launch for the remaining tiles may start on SMs that this one leaves
 
   float acc[NT / 2];
   if (warp == 0) {
@@ -150,32 +153,24 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
       for (int j = max(0, it - S); j < it; ++j) mbar_drain(&done[j % S], (j / S) & 1);
     }
   } else if (warp == 2) {
-    // ------------------------------------------------------------ packed weights
-    if (lane == 0) {
-      tma_prefetch_desc(&wmap);
-      int it = 0;
-      bool ok = true;
-      for (int t = first_tile; ok && t < tiles; t += tile_step) {
-        const int n0 = (t / p.tiles_m) * kW4gRows;
-        for (int k = k0; k < k1; k += kW4gPackedK, ++it) {
-          const int st = it % SP;
-          if (it >= SP && !mbar_wait(&empty_p[st], ((it / SP) - 1) & 1, &abort_flag)) {
-            ok = false;
-            break;
-          }
-          mbar_expect_tx(&full_p[st], kW4gPackedBytes);
-          tma_load_2d(packed + st * kW4gPackedBytes, &wmap, &full_p[st], k / 8, n0);
-        }
-      }
-      for (int j = max(0, it - SP); j < it; ++j) mbar_drain(&full_p[j % SP], (j / SP) & 1);
-    }
-  } else if (warp == 3) {
-    // ------------------------------------------------------------ scales and zero points
-    int ib = 0;
+    // ------------------------------------------------------------ scales, zero points, packed weights
+    // A batch of scales, then the boxes it belongs to: neither waits for the other's consumers
+    // longer than the rings are deep.
+    constexpr int kBatchK = kW4gScaleGroups * G;
+    static_assert(kBatchK % kW4gPackedK == 0, "whole boxes per batch");
+    auto box = [&](int i, int k, int n0) {  // the i-th box of this CTA
+      mbar_expect_tx(&full_p[i % SP], kW4gPackedBytes);
+      tma_load_2d(packed + (i % SP) * kW4gPackedBytes, &wmap, &full_p[i % SP], k / 8, n0);
+    };
+    int ib = 0, it = 0;
     bool ok = true;
+    int early = 0;  // boxes of the first tile that fill the ring before its scales are read
+    if (lane == 0 && first_tile < tiles)
+      for (; early < SP && k0 + early * kW4gPackedK < k1; ++early)
+        box(early, k0 + early * kW4gPackedK, (first_tile / p.tiles_m) * kW4gRows);
     for (int t = first_tile; ok && t < tiles; t += tile_step) {
       const int n0 = (t / p.tiles_m) * kW4gRows;
-      for (int b = 0; b < batches; ++b, ++ib) {
+      for (int b = 0; ok && b < batches; ++b, ++ib) {
         const int st = ib % kW4gScaleStages;
         ok = ib < kW4gScaleStages || mbar_wait(&empty_s[st], ((ib / kW4gScaleStages) - 1) & 1, &abort_flag);
         ok = __all_sync(0xffffffffu, ok);
@@ -199,44 +194,53 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full_s[st]);
+        if (lane == 0) {
+          mbar_arrive(&full_s[st]);
+          const int end = min(k1, k0 + (b + 1) * kBatchK);
+          for (int k = k0 + b * kBatchK; k < end; k += kW4gPackedK, ++it) {
+            if (it < early) continue;
+            if (it >= SP && !mbar_wait(&empty_p[it % SP], ((it / SP) - 1) & 1, &abort_flag)) {
+              ok = false;
+              break;
+            }
+            box(it, k, n0);
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issue (converged warp)
+    if (lane == 0) {
+      it = max(it, early);
+      for (int j = max(0, it - SP); j < it; ++j) mbar_drain(&full_p[j % SP], (j / SP) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1 || warp == 3) {
+    // ------------------------------------------------------------ MMA issue (converged warps)
     constexpr uint32_t idesc = idesc_bf16(kW4gRows, NT, false, false);
     const uint64_t desc0 = smem_desc(smem_u32(xs), 16, 1024, kSwizzle128B);
     const int mine = first_tile < tiles ? (tiles - first_tile + tile_step - 1) / tile_step : 0;
     const int total = mine * steps;  // steps of all this CTA's tiles
-    bool seen = false, ok = true;    // seen: the step's barrier was found complete during the step before
-    // Unrolled over the ring, so that descriptors and tensor-memory addresses are constants beside
-    // a uniform base.
+    const int turn = warp == 1 ? 0 : 1;
+    bool seen = false;               // the step's barrier was found complete during the step before
 #pragma unroll 1
-    for (int it0 = 0; ok && it0 < total; it0 += S) {
-      const uint32_t parity = (it0 / S) & 1;
+    for (int it = turn; it < total; it += 2) {
+      const int st = it % S;
+      if (!seen && !mbar_wait_fast(&ready[st], (it / S) & 1, &abort_flag)) break;
+      tc_fence_after();
+      seen = mbar_poll(&ready[(it + 2) % S], ((it + 2) / S) & 1);
+      const uint64_t b = desc0 + static_cast<uint64_t>((st * Shape::kXBytes) >> 4);
+      const uint32_t a = tmem_a + kW4gACols * st;
+      const uint32_t d = tmem + (it % kLag) * (GPS * NT);
+      // Past k's end the codes and activations are zeros: whole groups of them, never added.
 #pragma unroll
-      for (int st = 0; st < S; ++st) {
-        if (it0 + st >= total) break;
-        if (!seen && !mbar_wait_fast(&ready[st], parity, &abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        seen = mbar_poll(&ready[(st + 1) % S], st + 1 < S ? parity : parity ^ 1u);
-        const uint64_t b = desc0 + static_cast<uint64_t>((st * Shape::kXBytes) >> 4);
-        const uint32_t a = tmem_a + kW4gACols * st;
-        const uint32_t d = tmem + (st % kLag) * (GPS * NT);  // S is a multiple of kLag
-        // Past k's end the codes and activations are zeros: whole groups of them, never added.
-#pragma unroll
-        for (int j = 0; j < kStepMmas; ++j)
-          mma_ts_warp(d + (j / kGroupMmas) * NT, a + 8 * j,
-                      b + (j / 4) * static_cast<uint64_t>(Shape::kBoxBytes >> 4) + 2 * (j % 4), idesc,
-                      j % kGroupMmas != 0 ? 1u : 0u);
-        mma_commit_warp(&done[st]);
-      }
+      for (int j = 0; j < kStepMmas; ++j)
+        mma_ts_warp(d + (j / kGroupMmas) * NT, a + 8 * j,
+                    b + (j / 4) * static_cast<uint64_t>(Shape::kBoxBytes >> 4) + 2 * (j % 4), idesc,
+                    j % kGroupMmas != 0 ? 1u : 0u);
+      mma_commit_warp(&done[st]);
     }
-    mma_commit_warp(&drain_bar);  // nothing may still write tensor memory when it is freed
-    mbar_drain(&drain_bar, 0);
+    mma_commit_warp(&drain_bar[turn]);  // nothing may still write tensor memory when it is freed
+    mbar_drain(&drain_bar[turn], 0);
   } else if (warp >= kW4gFirstUnpack && warp < kW4gFirstAdd) {
     // ------------------------------------------------------------ codes -> bf16 A operand
     const int quad = warp & 3, r = quad * 32 + lane, turn = (warp - kW4gFirstUnpack) >> 2;
@@ -423,6 +427,7 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
     tc_fence_after();
     tmem_dealloc(tmem, kW4gTmemCols);
   }
+  if (p.tile0 > 0) pdl_wait();  // the launch ahead (the other tiles, same inputs) completes before this one
 }
 
 }  // namespace hb

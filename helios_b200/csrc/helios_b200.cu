@@ -140,7 +140,7 @@ int ensure_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 bool g_dec_smem[4][64], g_decp_smem[4][64], g_pre_smem[4][64], g_prx_smem[4][64], g_tick_smem[64], g_gemm_smem[64], g_argmax_smem[64];
-bool g_sparse_smem[4][64], g_control_smem[64], g_w4_smem[6][64], g_w4s_smem[18][64];
+bool g_sparse_smem[4][64], g_control_smem[64], g_w4_smem[6][64], g_w4s_smem[12][64];
 
 constexpr int kDefaultOverlapDecodeSms = 100;
 
@@ -180,21 +180,24 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t 
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// Launch with thread-block clusters of `cluster` CTAs along x.
+// Launch with thread-block clusters of `cluster` CTAs along x, if `early` before the kernel ahead of it
+// in the stream has finished (see launch_pdl).
 template <typename... Params, typename... Args>
 cudaError_t launch_cluster(void (*kernel)(Params...), dim3 grid, dim3 block, unsigned cluster, size_t smem,
-                           cudaStream_t stream, Args&&... args) {
+                           cudaStream_t stream, bool early, Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
@@ -216,28 +219,133 @@ int launch_fused_gemm(const typename Epi::Params& p, const CUtensorMap& amap, co
 template <int G, int NT, bool ZEROS>
 int launch_linear_w4(const hb::LinearW4Params& p, const CUtensorMap& xmap, const CUtensorMap& wmap, dim3 grid,
                      cudaStream_t stream) {
-  constexpr int slot = ((G == 128 ? 0 : G == 64 ? 1 : 2) * 3 + (NT == 4 ? 2 : NT - 1)) * 2 + (ZEROS ? 1 : 0);
+  constexpr int slot = ((G == 128 ? 0 : G == 64 ? 1 : 2) * 2 + NT - 1) * 2 + (ZEROS ? 1 : 0);
   constexpr int smem = hb::W4Stage<NT>::kSmem;
   if (int rc = ensure_smem(hb::linear_w4_kernel<G, NT, ZEROS>, smem, g_w4s_smem[slot])) return rc;
   const cudaError_t e =
-      launch_cluster(hb::linear_w4_kernel<G, NT, ZEROS>, grid, dim3(hb::kW4Threads), grid.x, smem, stream, p,
-                                       xmap, wmap);
+      launch_cluster(hb::linear_w4_kernel<G, NT, ZEROS>, grid, dim3(hb::kW4Threads), grid.x, smem, stream,
+                     false, p, xmap, wmap);
   if (e != cudaSuccess) return fail(HB_ERR_CUDA, "linear_w4_kernel: %s", cudaGetErrorString(e));
   return check_launch("linear_w4_kernel");
 }
 
+// The warp-MMA projection (linear_w4.cuh).
+int run_linear_w4(const hb::LinearW4Params& p, int group, cudaStream_t stream) {
+  const int nt = p.m <= 8 ? 1 : 2;
+  const int tiles = (p.n + hb::kW4Rows - 1) / hb::kW4Rows, token_tiles = (p.m + 8 * nt - 1) / (8 * nt);
+  // K splits, where one wave of CTAs holds them (with some room, as clusters do not fill every SM):
+  // the fewest that share the stages out as evenly as any.
+  const int stages = (p.k + hb::kW4StageK - 1) / hb::kW4StageK;
+  const int64_t wave = 148 * (nt == 1 ? hb::W4Stage<1>::kPerSm : hb::W4Stage<2>::kPerSm);
+  int splits = 1;
+  for (int s = 2; s <= hb::kW4MaxSplits; ++s)
+    if (static_cast<int64_t>(tiles) * token_tiles * s * 10 <= wave * 9 && (stages + s - 1) / s < (stages + splits - 1) / splits)
+      splits = s;
+  const dim3 grid(splits, tiles, token_tiles);
+  CUtensorMap xmap, wmap;
+  if (int rc = encode_2d(&xmap, p.x, p.k, p.m, static_cast<uint64_t>(p.x_stride) * 2, 64, 8 * nt)) return rc;
+  if (int rc = encode_packed(&wmap, p.packed, p.k / 8, p.n, hb::kW4Rows)) return rc;
+#define HB_W4_ZEROS(G, NT)                                                        \
+  return p.zeros != nullptr ? launch_linear_w4<G, NT, true>(p, xmap, wmap, grid, stream) \
+                            : launch_linear_w4<G, NT, false>(p, xmap, wmap, grid, stream)
+#define HB_W4_GROUP(G)                 \
+  do {                                 \
+    if (nt == 1) HB_W4_ZEROS(G, 1);    \
+    HB_W4_ZEROS(G, 2);                 \
+  } while (0)
+  if (group == 128) HB_W4_GROUP(128);
+  if (group == 64) HB_W4_GROUP(64);
+  HB_W4_GROUP(32);
+#undef HB_W4_GROUP
+#undef HB_W4_ZEROS
+}
+
+// Clusters of `size` CTAs of a kernel that run at once on this device (asked once).
+template <typename K>
+int max_clusters(K kernel, int size, unsigned threads, size_t smem, int (&known)[64][9]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (known[dev][size] == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+    known[dev][size] = n > 0 ? n : -1;
+  }
+  return known[dev][size];
+}
+
+int g_w4_clusters[6][64][9];
+
 template <int G, int NT>
-int launch_gemm_w4(const hb::GemmW4Params& p, const CUtensorMap& xmap, const CUtensorMap& wmap, int splits,
-                   cudaStream_t stream) {
+int launch_gemm_w4(hb::GemmW4Params p, int tiles, const CUtensorMap& xmap, const CUtensorMap& wmap, cudaStream_t stream) {
   constexpr int slot = (G == 128 ? 0 : G == 64 ? 1 : 2) * 2 + (NT == 128 ? 1 : 0);
   constexpr int smem = hb::GemmW4Shape<NT>::kSmem;
   if (int rc = ensure_smem(hb::gemm_w4_kernel<G, NT>, smem, g_w4_smem[slot])) return rc;
-  const int tiles = p.tiles_m * p.tiles_n;
-  const unsigned grid = splits > 1 ? tiles * splits : std::min(tiles, sm_count());
-  const cudaError_t e = launch_cluster(hb::gemm_w4_kernel<G, NT>, dim3(grid), dim3(hb::kW4gThreads), splits, smem, stream,
-                                       p, xmap, wmap);
-  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "gemm_w4_kernel: %s", cudaGetErrorString(e));
-  return check_launch("gemm_w4_kernel");
+  const int units = (p.k + 127) / 128, sms = sm_count();
+  if (sms <= 0) return fail(HB_ERR_CUDA, "cannot read the SM count");
+  // K splits of n tiles: rounds of clusters times their steps of 128 k's, with six steps' time for a
+  // round's start and sum (without splits a CTA walks its tiles in one go).
+  struct Plan {
+    int splits;
+    int64_t cost;
+  };
+  auto plan = [&](int n) {
+    Plan best{1, static_cast<int64_t>((n + sms - 1) / sms) * units + 6};
+    for (int s = 2; s <= 8 && s <= units; ++s) {
+      const int at_once = max_clusters(hb::gemm_w4_kernel<G, NT>, s, hb::kW4gThreads, smem, g_w4_clusters[slot]);
+      if (at_once <= 0) continue;
+      const int64_t cost = static_cast<int64_t>((n + at_once - 1) / at_once) * ((units + s - 1) / s + 6);
+      if (cost < best.cost) best = {s, cost};
+    }
+    return best;
+  };
+  auto launch = [&](int first, int n, int splits) {  // a second launch may start beside the first
+    p.tile0 = first;
+    p.tiles = n;
+    const unsigned grid = splits > 1 ? n * splits : std::min(n, sms);
+    const cudaError_t e = launch_cluster(hb::gemm_w4_kernel<G, NT>, dim3(grid), dim3(hb::kW4gThreads), splits, smem,
+                                         stream, first > 0, p, xmap, wmap);
+    if (e != cudaSuccess) return fail(HB_ERR_CUDA, "gemm_w4_kernel: %s", cudaGetErrorString(e));
+    return check_launch("gemm_w4_kernel");
+  };
+  // Tiles beyond the last whole round of SMs run as a launch of their own where splitting their k's
+  // is sooner done than a round for them (19456 weight rows and 61 tokens are 152 tiles: 29.8 us in
+  // two rounds).
+  const Plan whole = plan(tiles);
+  const int over = tiles % sms, rounds = tiles / sms;
+  if (rounds > 0 && over > 0) {
+    const Plan rest = plan(over);
+    if (static_cast<int64_t>(rounds) * units + 6 + 2 + rest.cost < whole.cost) {
+      if (int rc = launch(0, tiles - over, 1)) return rc;
+      return launch(tiles - over, over, rest.splits);
+    }
+  }
+  return launch(0, tiles, whole.splits);
+}
+
+// The tcgen05 projection (gemm_w4.cuh).
+int run_gemm_w4(const hb::LinearW4Params& p, int group, cudaStream_t stream) {
+  // Smaller groups need more accumulators per step: tiles of 64 tokens.
+  const int tile_tokens = p.m <= 64 || group != 128 ? 64 : 128;
+  const int64_t tiles_m = (p.m + tile_tokens - 1) / tile_tokens, tiles = tiles_m * ((p.n + hb::kW4gRows - 1) / hb::kW4gRows);
+  if (tiles > (1 << 24)) return fail(HB_ERR_UNSUPPORTED, "4-bit projection: %d x %d outputs are too many", p.m, p.n);
+  const hb::GemmW4Params g{p.scales, p.zeros, p.out, p.m, p.n, p.k, static_cast<int32_t>(tiles_m), 0, 0};
+  const int n = static_cast<int>(tiles);
+  CUtensorMap xmap, wmap;
+  if (int rc = encode_2d(&xmap, p.x, p.k, p.m, static_cast<uint64_t>(p.x_stride) * 2, hb::kW4gBoxK, tile_tokens)) return rc;
+  if (int rc = encode_packed(&wmap, p.packed, p.k / 8, p.n, hb::kW4gRows)) return rc;
+  if (group == 64) return launch_gemm_w4<64, 64>(g, n, xmap, wmap, stream);
+  if (group == 32) return launch_gemm_w4<32, 64>(g, n, xmap, wmap, stream);
+  return tile_tokens == 64 ? launch_gemm_w4<128, 64>(g, n, xmap, wmap, stream) : launch_gemm_w4<128, 128>(g, n, xmap, wmap, stream);
 }
 
 // RMSNorm launch: a CTA per row for few rows or hidden beyond 4096, else a warp per row.
@@ -820,53 +928,7 @@ int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const in
     return fail(HB_ERR_INVALID, "4-bit projection pointers must be non-null, x rows and packed 16-byte aligned");
   hb::LinearW4Params p{static_cast<const __nv_bfloat16*>(x), x_stride, reinterpret_cast<const uint32_t*>(packed),
                        static_cast<const __nv_bfloat16*>(scales), zeros, static_cast<__nv_bfloat16*>(out), m, n, k};
-  if (m > 32) {
-    // Smaller groups need more accumulators per step: tiles of 64 tokens.
-    const int tile_tokens = m <= 64 || group != 128 ? 64 : 128;
-    const hb::GemmW4Params g{static_cast<const __nv_bfloat16*>(scales), zeros, static_cast<__nv_bfloat16*>(out), m, n, k,
-                             (m + tile_tokens - 1) / tile_tokens, (n + hb::kW4gRows - 1) / hb::kW4gRows};
-    if (static_cast<int64_t>(g.tiles_m) * g.tiles_n > (1 << 24))
-      return fail(HB_ERR_UNSUPPORTED, "4-bit projection: %d x %d outputs are too many", m, n);
-    CUtensorMap xmap, wmap;
-    if (int rc = encode_2d(&xmap, x, k, m, static_cast<uint64_t>(x_stride) * 2, hb::kW4gBoxK, tile_tokens)) return rc;
-    if (int rc = encode_packed(&wmap, packed, k / 8, n, hb::kW4gRows)) return rc;
-    int sms = sm_count();
-    int splits = 1;
-    for (int s = 2; s <= 8 && s * 128 <= k; ++s)
-      if (g.tiles_m * g.tiles_n * s <= sms) splits = s;
-    if (group == 64) return launch_gemm_w4<64, 64>(g, xmap, wmap, splits, stream);
-    if (group == 32) return launch_gemm_w4<32, 64>(g, xmap, wmap, splits, stream);
-    return tile_tokens == 64 ? launch_gemm_w4<128, 64>(g, xmap, wmap, splits, stream)
-                             : launch_gemm_w4<128, 128>(g, xmap, wmap, splits, stream);
-  }
-  const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
-  const int tiles = (n + hb::kW4Rows - 1) / hb::kW4Rows, token_tiles = (m + 8 * nt - 1) / (8 * nt);
-  // K splits, where one wave of CTAs holds them (with some room, as clusters do not fill every SM):
-  // the fewest that share the stages out as evenly as any.
-  const int stages = (k + hb::kW4StageK - 1) / hb::kW4StageK;
-  const int64_t wave = 148 * (nt == 1 ? hb::W4Stage<1>::kPerSm : nt == 2 ? hb::W4Stage<2>::kPerSm : hb::W4Stage<4>::kPerSm);
-  int splits = 1;
-  for (int s = 2; s <= hb::kW4MaxSplits; ++s)
-    if (static_cast<int64_t>(tiles) * token_tiles * s * 10 <= wave * 9 && (stages + s - 1) / s < (stages + splits - 1) / splits)
-      splits = s;
-  const dim3 grid(splits, tiles, token_tiles);
-  CUtensorMap xmap, wmap;
-  if (int rc = encode_2d(&xmap, x, k, m, static_cast<uint64_t>(x_stride) * 2, 64, 8 * nt)) return rc;
-  if (int rc = encode_packed(&wmap, packed, k / 8, n, hb::kW4Rows)) return rc;
-#define HB_W4_ZEROS(G, NT) \
-  return zeros != nullptr ? launch_linear_w4<G, NT, true>(p, xmap, wmap, grid, stream) \
-                          : launch_linear_w4<G, NT, false>(p, xmap, wmap, grid, stream)
-#define HB_W4_GROUP(G)                 \
-  do {                                 \
-    if (nt == 1) HB_W4_ZEROS(G, 1);    \
-    if (nt == 2) HB_W4_ZEROS(G, 2);    \
-    HB_W4_ZEROS(G, 4);                 \
-  } while (0)
-  if (group == 128) HB_W4_GROUP(128);
-  if (group == 64) HB_W4_GROUP(64);
-  HB_W4_GROUP(32);
-#undef HB_W4_GROUP
-#undef HB_W4_ZEROS
+  return m <= hb::kW4MaxTokens ? run_linear_w4(p, group, stream) : run_gemm_w4(p, group, stream);
 }
 
 int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_pages, int32_t page_size,
@@ -939,8 +1001,8 @@ int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* v
 #define HB_SPARSE(G)                                                                                          \
   do {                                                                                                        \
     if (int rc = ensure_smem(hb::sparse_attention_kernel<G>, most, g_sparse_smem[gs])) return rc;             \
-    e = launch_cluster(hb::sparse_attention_kernel<G>, grid, dim3(hb::kSparseThreads), ranks, smem, stream, p, kmap, \
-                       vmap);                                                                                 \
+    e = launch_cluster(hb::sparse_attention_kernel<G>, grid, dim3(hb::kSparseThreads), ranks, smem, stream, false,  \
+                       p, kmap, vmap);                                                                                 \
   } while (0)
   switch (group) {
     case 1: HB_SPARSE(1); break;

@@ -1,4 +1,4 @@
-// Projections with 4-bit weights and group scales, for the few token rows of a decode tick.
+// Projections with 4-bit weights and group scales, for the few token rows of a small decode tick.
 //
 //   out[t, n] = bf16( sum_g s[g, n] * sum_{k in group g} (q[n, k] - z[g, n]) * x[t, k] )
 //
@@ -48,14 +48,17 @@ constexpr int kW4Threads = 32 * (kW4Warps + 1);  // and the copying one
 constexpr int kW4Rows = 16 * kW4Tiles;  // weight rows per CTA
 constexpr int kW4StageK = 256;          // k's per stage: 128 bytes of a packed row
 constexpr int kW4MaxSplits = 8;
+// Token rows from which the tcgen05 kernel (gemm_w4.cuh) takes over. 19456 x 2560: 17.9 us at 16 rows
+// and 32.7 at 32 with two tiles more of tokens here, 23.1 there at 33; 2560 x 9728: 11.4, 18.4 and 16.1.
+constexpr int kW4MaxTokens = 16;
 
 template <int NT>
 struct W4Stage {
   static constexpr int kWeightBytes = kW4Rows * kW4StageK / 2;  // one box of 128-byte rows
   static constexpr int kBoxBytes = 8 * NT * 128;                // activations: a box per 64 k's
   static constexpr int kBytes = kWeightBytes + kW4StageK / 64 * kBoxBytes;
-  static constexpr int kStages = NT == 1 ? 5 : NT == 2 ? 4 : 3;
-  static constexpr int kSmem = kStages * kBytes + 1024;  // 61, 65 and 73 KB
+  static constexpr int kStages = NT == 1 ? 5 : 4;
+  static constexpr int kSmem = kStages * kBytes + 1024;  // 61 and 65 KB
   static constexpr int kPerSm = NT == 1 ? 3 : 2;         // CTAs that fit an SM, by registers
 };
 
