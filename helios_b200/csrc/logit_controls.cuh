@@ -168,11 +168,19 @@ __global__ void __launch_bounds__(kControlThreads, 2) logit_controls_kernel(Logi
     if (j0 + 1 < bias1) bias_next = p.bias_tokens[j0 + 1];
   }
   if (hist_len > 0 || bias1 > bias0) __syncthreads();
-  bool outside = false;  // a history entry that is no token
+  // Every CTA looks at every entry, so an entry's few instructions are what counts here: the
+  // atomic is predicated, and one maximum replaces a test of every entry (128 rows: 44.3 -> 43.1 us).
+  const uint32_t words0 = smem_u32(words);
+  unsigned largest = 0;  // entry, as unsigned: whether one is no token
   auto count = [&](int i, int token) {
     const unsigned at = static_cast<unsigned>(token) - static_cast<unsigned>(first);  // below the segment wraps round
-    outside |= static_cast<unsigned>(token) >= static_cast<unsigned>(p.vocab);
-    if (at < static_cast<unsigned>(n)) atomicAdd(&words[at], i < prompt_len ? 0x10000u : 1u);
+    largest = max(largest, static_cast<unsigned>(token));
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.lt.u32 p, %0, %1;\n\t"
+        "@p red.shared.add.u32 [%2], %3;\n\t}" ::"r"(at),
+        "r"(n), "r"(words0 + 4u * at), "r"(i < prompt_len ? 0x10000u : 1u)
+        : "memory");
   };
   for (int i0 = tid; i0 < pieces; i0 += kControlAhead * kControlThreads) {
 #pragma unroll
@@ -196,7 +204,7 @@ __global__ void __launch_bounds__(kControlThreads, 2) logit_controls_kernel(Logi
     const int i = tid < lead ? tid : hist_len - tail + tid - lead;
     count(i, hist[i]);
   }
-  if (first_cta && outside) raise_status(kStatusBadToken);
+  if (first_cta && largest >= static_cast<unsigned>(p.vocab)) raise_status(kStatusBadToken);
   // A list entry counts when its token is below the next entry's: ascending lists count whole,
   // of equal neighbours the last one does.
   for (int j = j0; j < bias1; j += kControlThreads) {
