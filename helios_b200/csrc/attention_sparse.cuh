@@ -107,6 +107,8 @@ __global__ void __launch_bounds__(kBoundsThreads) key_block_bounds_kernel(BlockB
   __shared__ uint4 other[kBoundsThreads / 64][2][16];  // a head's second warp: minima, maxima
   __shared__ int3 found[kBoundsThreads];               // page, first key in it, keys
   __shared__ int n_found;
+  pdl_wait();  // the keys, from the kernel ahead
+  pdl_trigger();
   for (int64_t t0 = blockIdx.x; t0 < p.tokens; t0 += static_cast<int64_t>(kBoundsThreads) * gridDim.x) {
     if (threadIdx.x == 0) n_found = 0;
     __syncthreads();
@@ -420,6 +422,8 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
   int* list = reinterpret_cast<int*>(smem + kDecRingBytes);  // [top] selected blocks, ascending
   int* where = list + p.top;                                 // [top] first pool token, -1: no page
   int* pages = where + p.top;                                // [width] the row's pages
+  pdl_wait();  // keys, bounds and queries, from the kernels ahead
+  pdl_trigger();
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());

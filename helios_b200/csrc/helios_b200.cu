@@ -140,7 +140,7 @@ int ensure_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 bool g_dec_smem[4][64], g_decp_smem[4][64], g_pre_smem[4][64], g_prx_smem[4][64], g_tick_smem[64], g_gemm_smem[64], g_argmax_smem[64];
-bool g_sparse_smem[4][64], g_control_smem[64], g_w4_smem[6][64], g_w4s_smem[12][64];
+bool g_sparse_smem[4][64], g_control_smem[64], g_w4_smem[6][64], g_w4s_smem[6][64];
 
 constexpr int kDefaultOverlapDecodeSms = 100;
 
@@ -216,49 +216,61 @@ int launch_fused_gemm(const typename Epi::Params& p, const CUtensorMap& amap, co
   return check_launch(what);
 }
 
-template <int G, int NT, bool ZEROS>
+template <int G, bool ZEROS>
 int launch_linear_w4(const hb::LinearW4Params& p, const CUtensorMap& xmap, const CUtensorMap& wmap, dim3 grid,
                      cudaStream_t stream) {
-  constexpr int slot = ((G == 128 ? 0 : G == 64 ? 1 : 2) * 2 + NT - 1) * 2 + (ZEROS ? 1 : 0);
-  constexpr int smem = hb::W4Stage<NT>::kSmem;
-  if (int rc = ensure_smem(hb::linear_w4_kernel<G, NT, ZEROS>, smem, g_w4s_smem[slot])) return rc;
-  const cudaError_t e =
-      launch_cluster(hb::linear_w4_kernel<G, NT, ZEROS>, grid, dim3(hb::kW4Threads), grid.x, smem, stream,
-                     false, p, xmap, wmap);
+  constexpr int slot = (G == 128 ? 0 : G == 64 ? 1 : 2) * 2 + (ZEROS ? 1 : 0);
+  constexpr int smem = hb::W4Stage::kSmem;
+  if (int rc = ensure_smem(hb::linear_w4_kernel<G, ZEROS>, smem, g_w4s_smem[slot])) return rc;
+  const cudaError_t e = launch_cluster(hb::linear_w4_kernel<G, ZEROS>, grid, dim3(hb::kW4Threads), grid.x, smem, stream,
+                                       false, p, xmap, wmap);
   if (e != cudaSuccess) return fail(HB_ERR_CUDA, "linear_w4_kernel: %s", cudaGetErrorString(e));
   return check_launch("linear_w4_kernel");
 }
 
-// The warp-MMA projection (linear_w4.cuh).
+template <int G, bool ZEROS>
+int launch_linear_w4_direct(const hb::LinearW4Params& p, unsigned tiles, unsigned warps, cudaStream_t stream) {
+  const cudaError_t e =
+      launch_pdl(hb::linear_w4_direct_kernel<G, ZEROS>, dim3(tiles), dim3(32 * warps), 0, stream, p);
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "linear_w4_direct_kernel: %s", cudaGetErrorString(e));
+  return check_launch("linear_w4_direct_kernel");
+}
+
+#define HB_W4_GROUPS(LAUNCH, ...)                                                                   \
+  do {                                                                                              \
+    const bool zeros = p.zeros != nullptr;                                                          \
+    if (group == 128) return zeros ? LAUNCH<128, true>(__VA_ARGS__) : LAUNCH<128, false>(__VA_ARGS__); \
+    if (group == 64) return zeros ? LAUNCH<64, true>(__VA_ARGS__) : LAUNCH<64, false>(__VA_ARGS__);    \
+    return zeros ? LAUNCH<32, true>(__VA_ARGS__) : LAUNCH<32, false>(__VA_ARGS__);                     \
+  } while (0)
+
+// The projection for the fewest tokens (linear_w4.cuh).
+int run_linear_w4_direct(const hb::LinearW4Params& p, int group, cudaStream_t stream) {
+  // As many warps per row tile as one SM holds of all tiles' (32 per SM), evenly loaded.
+  const int tiles = (p.n + 15) / 16, units = (p.k + 127) / 128;
+  const int want = std::max(hb::kW4DirectFewest, std::min(hb::kW4DirectWarps, 32 * 148 / tiles));
+  const int rounds = (units + want - 1) / want, warps = (units + rounds - 1) / rounds;
+  HB_W4_GROUPS(launch_linear_w4_direct, p, tiles, warps, stream);
+}
+
+// The warp-MMA projection with a ring (linear_w4.cuh).
 int run_linear_w4(const hb::LinearW4Params& p, int group, cudaStream_t stream) {
-  const int nt = p.m <= 8 ? 1 : 2;
-  const int tiles = (p.n + hb::kW4Rows - 1) / hb::kW4Rows, token_tiles = (p.m + 8 * nt - 1) / (8 * nt);
+  const int tiles = (p.n + hb::kW4Rows - 1) / hb::kW4Rows;
   // K splits, where one wave of CTAs holds them (with some room, as clusters do not fill every SM):
   // the fewest that share the stages out as evenly as any.
   const int stages = (p.k + hb::kW4StageK - 1) / hb::kW4StageK;
-  const int64_t wave = 148 * (nt == 1 ? hb::W4Stage<1>::kPerSm : hb::W4Stage<2>::kPerSm);
+  const int64_t wave = 148 * hb::W4Stage::kPerSm;
   int splits = 1;
   for (int s = 2; s <= hb::kW4MaxSplits; ++s)
-    if (static_cast<int64_t>(tiles) * token_tiles * s * 10 <= wave * 9 && (stages + s - 1) / s < (stages + splits - 1) / splits)
+    if (static_cast<int64_t>(tiles) * s * 10 <= wave * 9 && (stages + s - 1) / s < (stages + splits - 1) / splits)
       splits = s;
-  const dim3 grid(splits, tiles, token_tiles);
+  const dim3 grid(splits, tiles);
   CUtensorMap xmap, wmap;
-  if (int rc = encode_2d(&xmap, p.x, p.k, p.m, static_cast<uint64_t>(p.x_stride) * 2, 64, 8 * nt)) return rc;
+  if (int rc = encode_2d(&xmap, p.x, p.k, p.m, static_cast<uint64_t>(p.x_stride) * 2, 64, hb::kW4MaxTokens)) return rc;
   if (int rc = encode_packed(&wmap, p.packed, p.k / 8, p.n, hb::kW4Rows)) return rc;
-#define HB_W4_ZEROS(G, NT)                                                        \
-  return p.zeros != nullptr ? launch_linear_w4<G, NT, true>(p, xmap, wmap, grid, stream) \
-                            : launch_linear_w4<G, NT, false>(p, xmap, wmap, grid, stream)
-#define HB_W4_GROUP(G)                 \
-  do {                                 \
-    if (nt == 1) HB_W4_ZEROS(G, 1);    \
-    HB_W4_ZEROS(G, 2);                 \
-  } while (0)
-  if (group == 128) HB_W4_GROUP(128);
-  if (group == 64) HB_W4_GROUP(64);
-  HB_W4_GROUP(32);
-#undef HB_W4_GROUP
-#undef HB_W4_ZEROS
+  HB_W4_GROUPS(launch_linear_w4, p, xmap, wmap, grid, stream);
 }
+#undef HB_W4_GROUPS
 
 // Clusters of `size` CTAs of a kernel that run at once on this device (asked once).
 template <typename K>
@@ -928,6 +940,7 @@ int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const in
     return fail(HB_ERR_INVALID, "4-bit projection pointers must be non-null, x rows and packed 16-byte aligned");
   hb::LinearW4Params p{static_cast<const __nv_bfloat16*>(x), x_stride, reinterpret_cast<const uint32_t*>(packed),
                        static_cast<const __nv_bfloat16*>(scales), zeros, static_cast<__nv_bfloat16*>(out), m, n, k};
+  if (m <= hb::kW4DirectTokens) return run_linear_w4_direct(p, group, stream);
   return m <= hb::kW4MaxTokens ? run_linear_w4(p, group, stream) : run_gemm_w4(p, group, stream);
 }
 
@@ -948,7 +961,9 @@ int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_pages, i
   hb::BlockBoundsParams p{static_cast<const __nv_bfloat16*>(key_pool), static_cast<__nv_bfloat16*>(bounds), block_table,
                           cu_seq_q, seqused_k, token_row, num_rows, total_tokens, width,
                           static_cast<int32_t>(num_pages), page_size, kv_heads};
-  hb::key_block_bounds_kernel<<<std::min(total_tokens, hb::kBoundsCtas), hb::kBoundsThreads, 0, stream>>>(p);
+  const cudaError_t e = launch_pdl(hb::key_block_bounds_kernel, dim3(std::min(total_tokens, hb::kBoundsCtas)),
+                                   dim3(hb::kBoundsThreads), 0, stream, p);
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "key_block_bounds_kernel: %s", cudaGetErrorString(e));
   return check_launch("key_block_bounds_kernel");
 }
 
@@ -1001,8 +1016,8 @@ int hb_sparse_paged_attention(const void* q, const void* key_pool, const void* v
 #define HB_SPARSE(G)                                                                                          \
   do {                                                                                                        \
     if (int rc = ensure_smem(hb::sparse_attention_kernel<G>, most, g_sparse_smem[gs])) return rc;             \
-    e = launch_cluster(hb::sparse_attention_kernel<G>, grid, dim3(hb::kSparseThreads), ranks, smem, stream, false,  \
-                       p, kmap, vmap);                                                                                 \
+    e = launch_cluster(hb::sparse_attention_kernel<G>, grid, dim3(hb::kSparseThreads), ranks, smem, stream,   \
+                       true, p, kmap, vmap);                                                                  \
   } while (0)
   switch (group) {
     case 1: HB_SPARSE(1); break;
@@ -1046,8 +1061,10 @@ int hb_control_logits(const void* logits, int64_t row_stride, int32_t rows, int3
   const int most = hb::control_smem_bytes(hb::kControlMaxSegment, true, true);
   if (int rc = ensure_smem(hb::logit_controls_kernel, most, g_control_smem)) return rc;
   const dim3 grid((vocab + segment - 1) / segment, rows);
-  hb::logit_controls_kernel<<<grid, hb::kControlThreads,
-                              hb::control_smem_bytes(segment, history != nullptr, bias_offsets != nullptr), stream>>>(p);
+  const cudaError_t e =
+      launch_pdl(hb::logit_controls_kernel, grid, dim3(hb::kControlThreads),
+                 hb::control_smem_bytes(segment, history != nullptr, bias_offsets != nullptr), stream, p);
+  if (e != cudaSuccess) return fail(HB_ERR_CUDA, "logit_controls_kernel: %s", cudaGetErrorString(e));
   return check_launch("logit_controls_kernel");
 }
 

@@ -20,11 +20,13 @@
 // summed in a fresh fp32 accumulator and scaled once, in fp32, so the only rounding to bf16 is the
 // output's.
 //
-// A CTA has 64 weight rows, two warps for every 16, and all tokens of its tile. One more brings weights
-// and activations by TMA into a ring of stages of 256 k's, so that every SM keeps 190 KB and more
-// on the way whatever the others do. (One token, 19456 x 2560: 14.5 us with each warp loading its
-// own fragments, 13.9 with 16-byte asynchronous copies by all threads, 18.2 with bulk copies of
-// single rows.) A cluster of CTAs shares k where there are few weight rows.
+// Two kernels share this: up to 8 tokens warps load their own fragments (the second one below); from
+// 9 to 16, with twice the activations per weight, a ring filled by TMA brings both. There a CTA has
+// 64 weight rows, two warps for every 16, and all tokens; one more warp copies stages of 256 k's, so that
+// every SM keeps 130 KB on the way whatever the others do, and a cluster of CTAs shares k where there are
+// few weight rows. 16 tokens: 19456 x 2560 in 18.6 us (21.8 with each warp loading its own fragments),
+// 2560 x 9728 in 11.5 (17.9), 6144 x 2560 in 9.0 (8.8), 2560 x 4096 in 8.2 (8.7). Both kernels are bound
+// by latency (launch, first bytes, the sums over warps and CTAs) more than by HBM: 1.2 to 2.3 TB/s.
 #pragma once
 
 #include "hb_common.cuh"
@@ -48,18 +50,17 @@ constexpr int kW4Threads = 32 * (kW4Warps + 1);  // and the copying one
 constexpr int kW4Rows = 16 * kW4Tiles;  // weight rows per CTA
 constexpr int kW4StageK = 256;          // k's per stage: 128 bytes of a packed row
 constexpr int kW4MaxSplits = 8;
-// Token rows from which the tcgen05 kernel (gemm_w4.cuh) takes over. 19456 x 2560: 17.9 us at 16 rows
+// Most token rows here; the tcgen05 kernel (gemm_w4.cuh) has more. 19456 x 2560: 17.9 us at 16 rows
 // and 32.7 at 32 with two tiles more of tokens here, 23.1 there at 33; 2560 x 9728: 11.4, 18.4 and 16.1.
 constexpr int kW4MaxTokens = 16;
 
-template <int NT>
 struct W4Stage {
   static constexpr int kWeightBytes = kW4Rows * kW4StageK / 2;  // one box of 128-byte rows
-  static constexpr int kBoxBytes = 8 * NT * 128;                // activations: a box per 64 k's
+  static constexpr int kBoxBytes = kW4MaxTokens * 128;          // activations: a box per 64 k's
   static constexpr int kBytes = kWeightBytes + kW4StageK / 64 * kBoxBytes;
-  static constexpr int kStages = NT == 1 ? 5 : 4;
-  static constexpr int kSmem = kStages * kBytes + 1024;  // 61 and 65 KB
-  static constexpr int kPerSm = NT == 1 ? 3 : 2;         // CTAs that fit an SM, by registers
+  static constexpr int kStages = 4;
+  static constexpr int kSmem = kStages * kBytes + 1024;  // 65 KB
+  static constexpr int kPerSm = 2;                       // CTAs that fit an SM, by registers
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -125,13 +126,26 @@ __device__ __forceinline__ void shared_load(uint32_t src, uint32_t (&v)[WORDS]) 
   else
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(src));
 }
-// Grid (cluster of K splits, row tiles, token tiles). Rank r of a cluster has the stages r, r +
+template <int WORDS>
+__device__ __forceinline__ void global_load(const uint32_t* src, uint32_t* v) {
+  if constexpr (WORDS == 4) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(src));
+    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+  } else if constexpr (WORDS == 2) {
+    const uint2 q = __ldg(reinterpret_cast<const uint2*>(src));
+    v[0] = q.x, v[1] = q.y;
+  } else {
+    v[0] = __ldg(src);
+  }
+}
+// Grid (cluster of K splits, row tiles). Rank r of a cluster has the stages r, r +
 // splits, ...; the CTAs' sums are added in rank order, from shared memory, so results do not
 // depend on timing. Weight rows, tokens and k's past the end arrive as zeros.
-template <int G, int NT, bool ZEROS>
-__global__ void __launch_bounds__(kW4Threads, W4Stage<NT>::kPerSm) linear_w4_kernel(LinearW4Params p, const __grid_constant__ CUtensorMap xmap,
-                                                               const __grid_constant__ CUtensorMap wmap) {
-  using Stage = W4Stage<NT>;
+template <int G, bool ZEROS>
+__global__ void __launch_bounds__(kW4Threads, W4Stage::kPerSm)
+    linear_w4_kernel(LinearW4Params p, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+  using Stage = W4Stage;
+  constexpr int NT = kW4MaxTokens / 8;  // MMA tiles of tokens
   constexpr int WPG = G / 32;         // words of one group that a thread holds
   constexpr int GPT = kW4StageK / G / kW4Halves;  // groups per stage and warp
   constexpr int kTokens = 8 * NT, kStages = Stage::kStages;
@@ -145,7 +159,7 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage<NT>::kPerSm) linear_w4_ker
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, c4 = lane & 3;
   const int splits = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
-  const int row0 = blockIdx.y * kW4Rows, t0 = blockIdx.z * kTokens;
+  const int row0 = blockIdx.y * kW4Rows;
   const int all = (p.k + kW4StageK - 1) / kW4StageK;
   const int n = rank < all ? (all - rank + splits - 1) / splits : 0;  // this CTA's stages
   if (tid == 0) {
@@ -172,7 +186,7 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage<NT>::kPerSm) linear_w4_ker
         tma_load_2d_at(dst, &wmap, &full[st], k0 / 8, row0);
 #pragma unroll
         for (int b = 0; b < kW4StageK / 64; ++b)
-          tma_load_2d_at(dst + Stage::kWeightBytes + b * Stage::kBoxBytes, &xmap, &full[st], k0 + 64 * b, t0);
+          tma_load_2d_at(dst + Stage::kWeightBytes + b * Stage::kBoxBytes, &xmap, &full[st], k0 + 64 * b, 0);
       }
       for (int j = max(0, s - kStages); j < s; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
     }
@@ -285,7 +299,7 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage<NT>::kPerSm) linear_w4_ker
   }
   if (splits > 1) cluster_sync();
   else __syncthreads();
-  const int tokens = min(kTokens, p.m - t0);
+  const int tokens = p.m;
   // Every CTA finishes a share of the outputs, four rows at a time.
   const bool wide = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
   for (int i = rank * kW4Threads + tid; i < tokens * kW4Rows / 4; i += splits * kW4Threads) {
@@ -305,7 +319,7 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage<NT>::kPerSm) linear_w4_ker
         s.w += v[q].w;
       }
     const float o[4] = {s.x, s.y, s.z, s.w};
-    __nv_bfloat16* dst = p.out + static_cast<int64_t>(t0 + token) * p.n + row;
+    __nv_bfloat16* dst = p.out + static_cast<int64_t>(token) * p.n + row;
     if (wide) {
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
     } else {
@@ -315,6 +329,98 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage<NT>::kPerSm) linear_w4_ker
     }
   }
   if (splits > 1) cluster_sync();  // the sums stay until every CTA has read them
+}
+
+// Up to 8 tokens: no ring and no cluster. A CTA has 16 weight rows; each of its warps takes every
+// `warps`-th unit of 128 k's, loads the next one's weights and scales into registers when it has done
+// with one, and the warps' sums are added in shared memory, in warp order. Many warps keep the loads
+// on the way here, so registers count: 64 a thread, 32 warps per SM. With four units ahead in 124
+// registers 19456 x 2560 took 13.9 us, with prefetches into L2 12.3, with 40 registers 15.2, with two
+// chains of MMAs per sum 13.3, as it stands 11.0 (one token, weights from DRAM, 2.3 TB/s; the ring
+// kernel with one tile of tokens took 15.0); 6144 x 2560 5.2 (7.5), 2560 x 4096 5.2 (6.8), 2560 x 9728
+// 9.8 (10.1); 8 tokens 13.0 (15.2), 5.6 (7.8), 5.8 (7.2), 10.9 (10.7).
+constexpr int kW4DirectTokens = 8;
+constexpr int kW4DirectWarps = 16;  // at most
+constexpr int kW4DirectFewest = 5;  // where the units allow
+
+template <int G, bool ZEROS>
+__global__ void __launch_bounds__(32 * kW4DirectWarps, 2) linear_w4_direct_kernel(LinearW4Params p) {
+  constexpr int WPG = G / 32, GPU = 128 / G;  // words of a group that a thread holds, groups per unit
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, c4 = lane & 3;
+  const int warps = blockDim.x >> 5, row0 = blockIdx.x * 16;
+  const int ra = min(row0 + g4, p.n - 1), rb = min(row0 + g4 + 8, p.n - 1);
+  const int groups = p.k / G, units = (groups + GPU - 1) / GPU;
+  const uint32_t* wa = p.packed + static_cast<int64_t>(ra) * (p.k / 8) + WPG * c4;
+  const uint32_t* wb = p.packed + static_cast<int64_t>(rb) * (p.k / 8) + WPG * c4;
+  const __nv_bfloat16* x = p.x + min(g4, p.m - 1) * p.x_stride + 8 * WPG * c4;
+  uint32_t qa[4], qb[4];
+  __nv_bfloat16 sa[GPU], sb[GPU];
+  uint8_t za[GPU], zb[GPU];
+  auto load = [&](int unit) {
+#pragma unroll
+    for (int g = 0; g < GPU; ++g) {
+      const int group = unit * GPU + g;
+      if (group >= groups) continue;
+      const int64_t at = static_cast<int64_t>(group) * p.n;
+      global_load<WPG>(wa + group * (G / 8), &qa[g * WPG]);
+      global_load<WPG>(wb + group * (G / 8), &qb[g * WPG]);
+      sa[g] = p.scales[at + ra];
+      sb[g] = p.scales[at + rb];
+      if (ZEROS) {
+        za[g] = p.zeros[at + ra];
+        zb[g] = p.zeros[at + rb];
+      }
+    }
+  };
+  pdl_wait();  // the activations, from the kernel ahead (it may have written weights, too)
+  pdl_trigger();
+  load(warp);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int unit = warp; unit < units; unit += warps) {
+#pragma unroll
+    for (int g = 0; g < GPU; ++g) {
+      const int group = unit * GPU + g;
+      if (group >= groups) break;
+      const float fa = __bfloat162float(sa[g]), fb = __bfloat162float(sb[g]);
+      const float oa = ZEROS ? 128.f + (za[g] & 15) : 136.f, ob = ZEROS ? 128.f + (zb[g] & 15) : 136.f;
+      float part[4] = {0.f, 0.f, 0.f, 0.f}, ones[4] = {0.f, 0.f, 0.f, 0.f};
+      uint4 xv[WPG];
+#pragma unroll
+      for (int w = 0; w < WPG; ++w)
+        xv[w] = g4 < p.m ? *reinterpret_cast<const uint4*>(x + group * G + 8 * w) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < WPG; ++w) {
+        constexpr uint32_t kOne = 0x3F803F80u;
+        constexpr uint32_t one[4] = {kOne, kOne, kOne, kOne};
+        uint32_t a[4], b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a[e] = ((qa[g * WPG + w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
+          b[e] = ((qb[g * WPG + w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
+        }
+        const uint32_t a0[4] = {a[0], b[0], a[1], b[1]}, a1[4] = {a[2], b[2], a[3], b[3]};
+        mma_16816(part, a0, xv[w].x, xv[w].y);
+        mma_16816(ones, one, xv[w].x, xv[w].y);
+        mma_16816(part, a1, xv[w].z, xv[w].w);
+        mma_16816(ones, one, xv[w].z, xv[w].w);
+      }
+      acc[0] += fa * (part[0] - oa * ones[0]);
+      acc[1] += fa * (part[1] - oa * ones[1]);
+      acc[2] += fb * (part[2] - ob * ones[2]);
+      acc[3] += fb * (part[3] - ob * ones[3]);
+    }
+    load(unit + warps);
+  }
+  __shared__ float parts[kW4DirectWarps][16 * kW4DirectTokens];  // [token][row]
+#pragma unroll
+  for (int e = 0; e < 4; ++e) parts[warp][(2 * c4 + (e & 1)) * 16 + g4 + 8 * (e >> 1)] = acc[e];
+  __syncthreads();
+  for (int i = tid; i < p.m * 16; i += blockDim.x) {
+    float sum = parts[0][i];
+    for (int w = 1; w < warps; ++w) sum += parts[w][i];
+    const int row = row0 + i % 16;
+    if (row < p.n) p.out[static_cast<int64_t>(i / 16) * p.n + row] = __float2bfloat16_rn(sum);
+  }
 }
 
 }  // namespace hb

@@ -89,6 +89,8 @@ __global__ void __launch_bounds__(kControlThreads, 2) logit_controls_kernel(Logi
   const __nv_bfloat16* in = p.in + row * p.in_stride;
   __nv_bfloat16* out = p.out + row * p.out_stride;
 
+  pdl_wait();  // the logits, from the kernel ahead
+  pdl_trigger();
   const bool vec = ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   const bool in_place = in == out;
 
