@@ -20,12 +20,13 @@ import torch
 from helios_b200 import ops
 
 MAX_HISTORY = 65_535
+FP32_MAX, FP32_TINY = torch.finfo(torch.float32).max, torch.finfo(torch.float32).tiny
 
 
 @dataclass(frozen=True)
 class LogitControls:
     """One request's controls. ``slot`` is its ``TokenHistory`` slot, which the penalties need;
-    ``logit_bias`` maps token ids to biases; ``allowed`` is a bool tensor ``[V]`` or a packed mask
+    ``logit_bias`` maps token ids to biases (-inf bans a token); ``allowed`` is a bool tensor ``[V]`` or a packed mask
     (``pack_mask``), None for no mask."""
     repetition_penalty: float = 1.0
     frequency_penalty: float = 0.0
@@ -35,14 +36,15 @@ class LogitControls:
     slot: int | None = None
 
     def __post_init__(self) -> None:
-        if not 0 < self.repetition_penalty < math.inf:
-            raise ValueError("repetition_penalty must be positive and finite")
-        if not (math.isfinite(self.frequency_penalty) and math.isfinite(self.presence_penalty)):
-            raise ValueError("frequency_penalty and presence_penalty must be finite")
+        # The device holds all of these in fp32.
+        if not FP32_TINY <= self.repetition_penalty <= FP32_MAX:
+            raise ValueError("repetition_penalty must be positive and finite in fp32")
+        if not (abs(self.frequency_penalty) <= FP32_MAX and abs(self.presence_penalty) <= FP32_MAX):
+            raise ValueError("frequency_penalty and presence_penalty must be finite in fp32")
         if self.penalised and self.slot is None:
             raise ValueError("penalties need the request's TokenHistory slot")
-        if any(token < 0 or math.isnan(bias) for token, bias in self.logit_bias.items()):
-            raise ValueError("logit_bias maps token ids >= 0 to numbers")
+        if any(token < 0 or not (bias == -math.inf or abs(bias) <= FP32_MAX) for token, bias in self.logit_bias.items()):
+            raise ValueError("logit_bias maps token ids >= 0 to finite numbers or -inf")
 
     @property
     def penalised(self) -> bool:
@@ -104,7 +106,9 @@ class TokenHistory:
         return slot
 
     def append(self, slots: Sequence[int], ids: torch.Tensor | Sequence[int]) -> None:
-        """One token for each of ``slots`` (distinct): ``ids`` on the device, or a list."""
+        """One token for each of ``slots`` (distinct): ``ids`` on the device, or a list. Ids on the device
+        are not looked at here: one that is no token (the -1 of a row in which nothing was allowed)
+        is flagged by the next ``control_rows`` that reads it, and counts for nothing."""
         slots = list(slots)
         if len(set(slots)) != len(slots):
             raise ValueError("a history slot takes one token at a time")

@@ -46,6 +46,12 @@ int check_launch(const char* what) {
   return HB_OK;
 }
 
+// Whether two ranges of memory share a byte.
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // ---- cuTensorMapEncodeTiled through the runtime's driver entry point (no -lcuda).
@@ -938,6 +944,8 @@ int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const in
   if (x == nullptr || packed == nullptr || scales == nullptr || out == nullptr || !aligned(x, 16) ||
       !aligned(packed, 16) || !aligned(scales, 2) || !aligned(out, 2) || x_stride % 8 != 0)
     return fail(HB_ERR_INVALID, "4-bit projection pointers must be non-null, x rows and packed 16-byte aligned");
+  if (overlap(x, 2 * ((m - 1) * x_stride + k), out, 2 * static_cast<int64_t>(m) * n))
+    return fail(HB_ERR_INVALID, "4-bit projection: x and out overlap");
   hb::LinearW4Params p{static_cast<const __nv_bfloat16*>(x), x_stride, reinterpret_cast<const uint32_t*>(packed),
                        static_cast<const __nv_bfloat16*>(scales), zeros, static_cast<__nv_bfloat16*>(out), m, n, k};
   if (m <= hb::kW4DirectTokens) return run_linear_w4_direct(p, group, stream);
@@ -1041,6 +1049,9 @@ int hb_control_logits(const void* logits, int64_t row_stride, int32_t rows, int3
   if (rows == 0) return HB_OK;
   if (logits == nullptr || out == nullptr) return fail(HB_ERR_INVALID, "null logits");
   if (logits == out && row_stride != out_stride) return fail(HB_ERR_INVALID, "in place needs equal row strides");
+  if (logits != out &&
+      overlap(logits, 2 * ((rows - 1) * row_stride + vocab), out, 2 * ((rows - 1) * out_stride + vocab)))
+    return fail(HB_ERR_INVALID, "out must be logits itself or apart from it");
   if (history != nullptr && (slots == nullptr || lengths == nullptr || prompt_lengths == nullptr || history_rows < 1 ||
                              history_width < 1))
     return fail(HB_ERR_INVALID, "a history needs its slots, lengths and prompt lengths");

@@ -118,12 +118,15 @@ class FeedForward(nn.Module):
         self.up = nn.Linear(config.hidden_size, config.hidden_dim, bias=False, dtype=config.dtype)
         self.down = nn.Linear(config.hidden_dim, config.hidden_size, bias=False, dtype=config.dtype)
         self._gate_up = _Fused(self.gate, self.up)
-        self.w4_gate_up: W4Linear | None = None  # set by quantize
+        self.w4_gate_up: W4Linear | None = None  # set by use_w4
         self.w4_down: W4Linear | None = None
 
-    def quantize(self, group_size: int, symmetric: bool) -> None:
-        self.w4_gate_up = W4Linear(quantize_w4(self._gate_up.get(), group_size, symmetric=symmetric))
-        self.w4_down = W4Linear(quantize_w4(self.down.weight, group_size, symmetric=symmetric))
+    def quantized(self, group_size: int, symmetric: bool) -> tuple[W4Linear, W4Linear]:
+        return (W4Linear(quantize_w4(self._gate_up.get(), group_size, symmetric=symmetric)),
+                W4Linear(quantize_w4(self.down.weight, group_size, symmetric=symmetric)))
+
+    def use_w4(self, gate_up: W4Linear, down: W4Linear) -> None:
+        self.w4_gate_up, self.w4_down = gate_up, down
         self._gate_up = None
         _drop(self.gate, self.up, self.down)
 
@@ -162,12 +165,15 @@ class GroupedQueryAttention(nn.Module):
         self.q_norm = RMSNorm(config.head_dim, config.rms_norm_eps)
         self.k_norm = RMSNorm(config.head_dim, config.rms_norm_eps)
         self._qkv = _Fused(self.query, self.key, self.value)
-        self.w4_qkv: W4Linear | None = None  # set by quantize
+        self.w4_qkv: W4Linear | None = None  # set by use_w4
         self.w4_output: W4Linear | None = None
 
-    def quantize(self, group_size: int, symmetric: bool) -> None:
-        self.w4_qkv = W4Linear(quantize_w4(self._qkv.get(), group_size, symmetric=symmetric))
-        self.w4_output = W4Linear(quantize_w4(self.output.weight, group_size, symmetric=symmetric))
+    def quantized(self, group_size: int, symmetric: bool) -> tuple[W4Linear, W4Linear]:
+        return (W4Linear(quantize_w4(self._qkv.get(), group_size, symmetric=symmetric)),
+                W4Linear(quantize_w4(self.output.weight, group_size, symmetric=symmetric)))
+
+    def use_w4(self, qkv: W4Linear, output: W4Linear) -> None:
+        self.w4_qkv, self.w4_output = qkv, output
         self._qkv = None
         _drop(self.query, self.key, self.value, self.output)
 
@@ -234,9 +240,12 @@ class Qwen3Model(nn.Module):
         for block in self.blocks:
             if block.feed_forward.w4_gate_up is not None:
                 raise RuntimeError("The model's weights are already quantized.")
-        for block in self.blocks:
-            block.attention.quantize(group_size, symmetric)
-            block.feed_forward.quantize(group_size, symmetric)
+        # All of them before the first is replaced: a weight that is refused leaves the model as it was.
+        held = [(block.attention.quantized(group_size, symmetric), block.feed_forward.quantized(group_size, symmetric))
+                for block in self.blocks]
+        for block, (attention, feed_forward) in zip(self.blocks, held):
+            block.attention.use_w4(*attention)
+            block.feed_forward.use_w4(*feed_forward)
         if self._graphs is not None:  # captured ticks run the freed weights
             self.enable_cuda_graphs(self._graphs.max_graphs)
 

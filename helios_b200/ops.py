@@ -275,7 +275,7 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
     in the low half, odd i's in the high half, see hb_linear_w4), ``scales`` bf16 ``[k / group, n]``,
     ``zeros`` uint8 ``[k / group, n]`` (None: 8); groups of 32, 64 or 128. ``x`` may have any row
     stride that keeps its rows 16-byte aligned. ``helios_b200.w4.quantize_w4`` makes the three
-    tensors from a weight. Returns ``out``, or a new tensor."""
+    tensors from a weight. Returns ``out`` (apart from ``x``), or a new tensor."""
     dev = x.device
     if not (x.is_cuda and x.dtype is BF16 and packed.dtype is I32 and scales.dtype is BF16 and packed.device == dev
             and scales.device == dev and packed.is_contiguous() and scales.is_contiguous() and x.dim() == 2
@@ -416,7 +416,8 @@ def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
         out = torch.empty_like(q)
     _call(lib().hb_sparse_paged_attention, "hb_sparse_paged_attention", dev, q.data_ptr(), key_pool.data_ptr(),
           value_pool.data_ptr(), bounds.data_ptr(), pages, page, block_table.data_ptr(), width, seqused_k.data_ptr(),
-          None if cu_seq_q is None else cu_seq_q.data_ptr(), rows, heads, kv_heads, dim, top_blocks, sink_blocks, recent_blocks, dim ** -0.5 if scale is None else scale,
+          None if cu_seq_q is None else cu_seq_q.data_ptr(), rows, heads, kv_heads, dim, top_blocks, sink_blocks,
+          recent_blocks, dim ** -0.5 if scale is None else scale,
           None if selected is None else selected.data_ptr(), out.data_ptr())
     return out
 

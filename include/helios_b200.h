@@ -251,7 +251,8 @@ HB_API int hb_lm_head_argmax(const void* x, int32_t m, int32_t k, const void* we
  * [n][k / 8]: word c of a row holds i = 8c .. 8c + 7, the even i in its low 16 bits and the odd
  * i in its high 16 bits, four bits each in ascending i; scales bf16 [k / group][n]; zeros uint8
  * [k / group][n] with values 0 .. 15 (the low four bits are used), null for 8 everywhere; group
- * 32, 64 or 128, k a multiple of it; out bf16 [m][n].
+ * 32, 64 or 128, k a multiple of it; out bf16 [m][n], apart from x. Sums are in fp32; a row of x
+ * with an infinity or a NaN gives NaN where the formula gives either (its other rows are unaffected).
  */
 HB_API int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const int32_t* packed,
                         const void* scales, const uint8_t* zeros, int32_t n, int32_t group, void* out,
@@ -306,7 +307,8 @@ HB_API int hb_sparse_paged_attention(const void* q, const void* key_pool, const 
  *                   skipped and flagged (HB_STATUS_BAD_TOKEN)
  *   mask            int32 [masks][ceil(vocab / 32)], bit i of word c allows token 32c + i; row r
  *                   uses mask mask_rows[r] (-1: none). A mask without a token leaves a row of -inf.
- * out bf16 rows out_stride apart, or logits itself (then only changed values are written).
+ * out bf16 rows out_stride apart, or logits itself (then only changed values are written);
+ * anything that overlaps logits otherwise is refused.
  */
 HB_API int hb_control_logits(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab,
                              const float* repetition, const float* frequency, const float* presence,

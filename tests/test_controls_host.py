@@ -91,3 +91,12 @@ def test_pool_bounds_cover_keys_appended_before():
     first = pool.bounds
     pool.enable_key_bounds()
     assert pool.bounds is first
+
+
+@pytest.mark.parametrize("bad", [dict(repetition_penalty=1e39, slot=0), dict(repetition_penalty=1e-50, slot=0),
+                                 dict(frequency_penalty=-1e39, slot=0), dict(presence_penalty=math.nan, slot=0),
+                                 dict(logit_bias={3: math.inf}), dict(logit_bias={3: 1e39})])
+def test_settings_that_fp32_does_not_hold(bad):
+    with pytest.raises(ValueError):
+        LogitControls(**bad)
+    assert LogitControls(logit_bias={3: -math.inf}).logit_bias[3] == -math.inf

@@ -244,3 +244,13 @@ def test_refusals():
     with pytest.raises(ValueError):
         ops.control_logits(x.t())
     assert _native.device_status() == 0
+
+
+def test_outputs_over_part_of_the_logits_are_refused():
+    memory = torch.zeros(4 * 100 + 8, dtype=torch.bfloat16, device=DEV)
+    x = memory[:400].view(4, 100)
+    for out in (memory[8:].view(4, 100), memory[:300].view(3, 100)):
+        with pytest.raises(ValueError):
+            ops.control_logits(x if out.shape[0] == 4 else memory[100:400].view(3, 100), out=out)
+    assert torch.equal(ops.control_logits(x[:2], out=x[2:]), x[:2])
+    assert _native.device_status() == 0

@@ -301,3 +301,14 @@ def test_refusals():
     with pytest.raises(ValueError):
         ops.key_block_bounds(keys, bounds, bt, used, used, used)
     assert _native.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_output_in_place_of_the_queries(rows):
+    keys, values, g = pool(4, 2, 16)
+    keys, values = keys.to(DEV), values.to(DEV)
+    bt = table([900], 4, g).to(DEV).repeat(rows, 1)
+    q = torch.randn(rows, 8, 128, generator=g).to(torch.bfloat16).to(DEV)
+    used = torch.full((rows,), 900, dtype=torch.int32, device=DEV)
+    want = ops.sparse_paged_attention(q, keys, values, whole_bounds(keys), bt, used, top_blocks=6)
+    assert torch.equal(ops.sparse_paged_attention(q, keys, values, whole_bounds(keys), bt, used, q, top_blocks=6), want)

@@ -6,6 +6,8 @@ import pytest
 import torch
 
 from helios_b200 import _native, ops
+from helios_b200.config import Qwen3Config
+from helios_b200.model import Qwen3Model
 from helios_b200.w4 import dequantize_w4, pack_w4, quantize_w4, unpack_w4
 
 
@@ -68,3 +70,34 @@ def test_projection_refusals():
     w = quantize_w4(torch.ones(8, 128))
     with pytest.raises(ValueError, match="CUDA"):
         ops.linear_w4(torch.zeros(2, 128, dtype=torch.bfloat16), *w)
+
+
+def test_overlapping_output_is_refused():
+    lib = _native.load()
+    base = 1 << 20  # never read: every call here is refused before a launch
+
+    def call(x, out, stride=256, m=2, n=8):
+        return lib.hb_linear_w4(ctypes.c_void_p(base + x), stride, m, 256, ctypes.c_void_p(base), ctypes.c_void_p(base),
+                                None, n, 128, ctypes.c_void_p(base + out), None)
+
+    for x, out, stride in ((0, 0, 256), (0, 1022, 256), (0, 1534, 512), (30, 0, 256), (16, 0, 256)):
+        assert call(x, out, stride) == _native.HB_ERR_INVALID, (x, out)
+    assert call(0, 1022) == _native.HB_ERR_INVALID and "overlap" in _native.last_error()
+
+
+@pytest.mark.parametrize("fault", ["size", "value"])
+def test_a_refused_weight_leaves_the_model_as_it_was(fault):
+    config = Qwen3Config(vocab_size=64, hidden_size=128, hidden_dim=192 if fault == "size" else 256, n_layers=2,
+                         n_heads=2, n_kv_heads=1, head_dim=64, context_length=64)
+    model = Qwen3Model(config)
+    if fault == "value":
+        with torch.no_grad():
+            model.blocks[1].feed_forward.down.weight[0, 0] = float("inf")
+    with pytest.raises(ValueError):
+        model.quantize_weights(128)
+    for block in model.blocks:
+        assert block.attention.w4_qkv is None and block.feed_forward.w4_down is None
+        assert block.attention.output.weight.numel() and block.feed_forward.down.weight.numel()
+    if fault == "size":
+        model.quantize_weights(64)
+        assert all(block.feed_forward.w4_down is not None for block in model.blocks)
