@@ -32,3 +32,36 @@ def test_matches_the_formula(m, k, n, group, zeros):
     got = ops.linear_w4(x, *w, out=out[1:m + 1])
     assert ((got.double() - y).abs() <= tol).all()
     assert (out[0] == 3).all() and (out[m + 1] == 3).all()
+
+
+@pytest.mark.parametrize("m,n", [(1, 512), (8, 512), (12, 512), (96, 512), (61, 19456)])
+def test_chains_wait_for_their_inputs(m, n):
+    """Twelve projections, each of the one before, into two buffers in turn: queued at once, and
+    replayed from a graph, they give what they give one by one."""
+    k = 256
+    g = torch.Generator(device=DEV).manual_seed(m)
+    codes = torch.randint(0, 16, (n, k), generator=g, device=DEV)
+    scales = (torch.rand(k // 64, n, generator=g, device=DEV) * 0.02 + 1e-3).to(torch.bfloat16)
+    packed = pack_w4(codes)
+    start = torch.randn(m, k, generator=g, device=DEV).to(torch.bfloat16)
+    buffers = [torch.zeros(m, n, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+
+    def chain(x, between=lambda: None):
+        for i in range(12):
+            x = ops.linear_w4(x, packed, scales, None, buffers[i % 2])[:, n - k:]
+            between()
+        return x.clone()
+
+    want = chain(start, torch.cuda.synchronize)
+    assert want.isfinite().all() and want.abs().amax() > 0
+    for _ in range(3):
+        assert torch.equal(chain(start), want)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = chain(start)
+    for _ in range(3):
+        for b in buffers:
+            b.zero_()
+        graph.replay()
+        assert torch.equal(got, want)
