@@ -43,7 +43,8 @@ class LogitControls:
             raise ValueError("frequency_penalty and presence_penalty must be finite in fp32")
         if self.penalised and self.slot is None:
             raise ValueError("penalties need the request's TokenHistory slot")
-        if any(token < 0 or not (bias == -math.inf or abs(bias) <= FP32_MAX) for token, bias in self.logit_bias.items()):
+        if any(token < 0 or not (bias == -math.inf or abs(bias) <= FP32_MAX)
+               for token, bias in self.logit_bias.items()):
             raise ValueError("logit_bias maps token ids >= 0 to finite numbers or -inf")
 
     @property
@@ -178,7 +179,8 @@ def control_rows(logits: torch.Tensor, controls: Sequence[LogitControls | None],
                 which.append(-1)
                 continue
             if id(c.allowed) not in seen:  # rows that share a mask object share its words
-                mask = pack_mask(c.allowed) if c.allowed.dtype == torch.bool and c.allowed.shape == (vocab,) else c.allowed
+                whole = c.allowed.dtype == torch.bool and c.allowed.shape == (vocab,)
+                mask = pack_mask(c.allowed) if whole else c.allowed
                 if mask.dtype != torch.int32 or mask.shape != (words,):
                     raise ValueError("allowed must be bool [V] or packed int32 [ceil(V / 32)]")
                 seen[id(c.allowed)] = len(masks)

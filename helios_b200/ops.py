@@ -227,20 +227,22 @@ def _together(device: torch.device, **tensors: torch.Tensor | None) -> None:
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _call(fn, name: str, device: torch.device, *args) -> None:
-    """Run an entry point on ``device``'s current stream, with that device current."""
-    if _get_device() == device.index:
-        rc = fn(*args, _stream(device))
+def _call(fn, name: str, device: int, *args) -> None:
+    """Run an entry point on the current stream of CUDA device ``device``, with that device current."""
+    stream = _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    if _get_device() == device:
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
+            rc = fn(*args, stream)
     if rc:
         _native.check(rc, name)
 
 
 # The operators below test their arguments in one expression, which is all that a call in order
 # pays for (each _need costs 0.3 us of host time, more than a decode step's smallest kernels can
-# hide); only when it fails, a second pass finds out which argument to name.
+# hide; get_device(), -1 for host tensors, costs half of comparing devices); only when it fails, a
+# second pass finds out which argument to name.
 I32, F32 = torch.int32, torch.float32
 
 
@@ -276,18 +278,18 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
     ``zeros`` uint8 ``[k / group, n]`` (None: 8); groups of 32, 64 or 128. ``x`` may have any row
     stride that keeps its rows 16-byte aligned. ``helios_b200.w4.quantize_w4`` makes the three
     tensors from a weight. Returns ``out`` (apart from ``x``), or a new tensor."""
-    dev = x.device
-    if not (x.is_cuda and x.dtype is BF16 and packed.dtype is I32 and scales.dtype is BF16 and packed.device == dev
-            and scales.device == dev and packed.is_contiguous() and scales.is_contiguous() and x.dim() == 2
+    dev = x.get_device()
+    if not (x.is_cuda and x.dtype is BF16 and packed.dtype is I32 and scales.dtype is BF16
+            and packed.get_device() == dev and scales.get_device() == dev and packed.is_contiguous() and scales.is_contiguous() and x.dim() == 2
             and packed.dim() == 2 and scales.dim() == 2):
         _refuse_linear_w4(x, packed, scales, zeros, out)
     m, k = x.shape
     n, words = packed.shape
     groups, scale_n = scales.shape
     if not (words * 8 == k and scale_n == n and groups and k % groups == 0 and x.stride(1) == 1
-            and (zeros is None or (zeros.dtype is torch.uint8 and zeros.device == dev and zeros.is_contiguous()
+            and (zeros is None or (zeros.dtype is torch.uint8 and zeros.get_device() == dev and zeros.is_contiguous()
                                    and zeros.shape == scales.shape))
-            and (out is None or (out.dtype is BF16 and out.device == dev and out.is_contiguous()
+            and (out is None or (out.dtype is BF16 and out.get_device() == dev and out.is_contiguous()
                                  and out.shape == (m, n)))):
         _refuse_linear_w4(x, packed, scales, zeros, out)
     if out is None:
@@ -327,11 +329,11 @@ def key_block_bounds(key_pool: torch.Tensor, bounds: torch.Tensor, block_table: 
     ``key_pool [pages, page, Hkv, d]`` and ``bounds [pages, Hkv, page / 64, 2, d]``, with the tick's
     ``block_table [rows, width]``, ``cu_seq_q [rows + 1]``, ``seqused_k [rows]`` and ``token_row
     [tokens]`` (all int32). Only blocks holding new positions are written. Returns ``bounds``."""
-    dev = key_pool.device
+    dev = key_pool.get_device()
     if not (key_pool.is_cuda and key_pool.dtype is BF16 and bounds.dtype is BF16 and block_table.dtype is I32
-            and cu_seq_q.dtype is I32 and seqused_k.dtype is I32 and token_row.dtype is I32 and bounds.device == dev
-            and block_table.device == dev and cu_seq_q.device == dev and seqused_k.device == dev
-            and token_row.device == dev and key_pool.is_contiguous() and bounds.is_contiguous()
+            and cu_seq_q.dtype is I32 and seqused_k.dtype is I32 and token_row.dtype is I32
+            and bounds.get_device() == dev and block_table.get_device() == dev and cu_seq_q.get_device() == dev and seqused_k.get_device() == dev
+            and token_row.get_device() == dev and key_pool.is_contiguous() and bounds.is_contiguous()
             and block_table.is_contiguous() and cu_seq_q.is_contiguous() and seqused_k.is_contiguous()
             and token_row.is_contiguous() and key_pool.dim() == 4 and block_table.dim() == 2):
         _refuse_bounds(key_pool, bounds, block_table, cu_seq_q, seqused_k, token_row)
@@ -388,12 +390,12 @@ def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
     Returns ``out [rows, H, d]``, or a new tensor; a row without keys gives zeros. With ``cu_seq_q``
     (int32 ``[rows + 1]``) ``q`` and ``out`` are ``[tokens, H, d]``, row r's token is ``cu_seq_q[r]``, and
     rows with other than one token are left as ``out`` has them (it has to be given then)."""
-    dev = q.device
+    dev = q.get_device()
     refuse = (q, key_pool, value_pool, bounds, block_table, seqused_k, cu_seq_q, out, selected, top_blocks)
     if not (q.is_cuda and q.dtype is BF16 and key_pool.dtype is BF16 and value_pool.dtype is BF16
             and bounds.dtype is BF16 and block_table.dtype is I32 and seqused_k.dtype is I32
-            and key_pool.device == dev and value_pool.device == dev and bounds.device == dev
-            and block_table.device == dev and seqused_k.device == dev and q.is_contiguous()
+            and key_pool.get_device() == dev and value_pool.get_device() == dev and bounds.get_device() == dev
+            and block_table.get_device() == dev and seqused_k.get_device() == dev and q.is_contiguous()
             and key_pool.is_contiguous() and value_pool.is_contiguous() and bounds.is_contiguous()
             and block_table.is_contiguous() and seqused_k.is_contiguous() and q.dim() == 3 and key_pool.dim() == 4
             and block_table.dim() == 2):
@@ -404,13 +406,13 @@ def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
     rows, width = block_table.shape
     if not (value_pool.shape == pool_shape and dim == pool_dim and seqused_k.numel() == rows
             and (tokens == rows if cu_seq_q is None else
-                 cu_seq_q.dtype is I32 and cu_seq_q.device == dev and cu_seq_q.is_contiguous()
+                 cu_seq_q.dtype is I32 and cu_seq_q.get_device() == dev and cu_seq_q.is_contiguous()
                  and cu_seq_q.numel() == rows + 1 and out is not None)
             and bounds.shape == (pages, kv_heads, page // BLOCK_KEYS, 2, dim)
-            and (out is None or (out.dtype is BF16 and out.device == dev and out.is_contiguous()
+            and (out is None or (out.dtype is BF16 and out.get_device() == dev and out.is_contiguous()
                                  and out.shape == q.shape))
-            and (selected is None or (selected.dtype is I32 and selected.device == dev and selected.is_contiguous()
-                                      and selected.shape == (rows, kv_heads, top_blocks)))):
+            and (selected is None or (selected.dtype is I32 and selected.get_device() == dev
+                                      and selected.is_contiguous() and selected.shape == (rows, kv_heads, top_blocks)))):
         _refuse_sparse(*refuse)
     if out is None:
         out = torch.empty_like(q)
@@ -483,13 +485,13 @@ def control_logits(logits: torch.Tensor, *, repetition: torch.Tensor | None = No
     slot -1: none). ``bias``: int32 offsets ``[rows + 1]``, int32 tokens (ascending within a row) and
     fp32 values. ``mask`` int32 ``[masks, ceil(V / 32)]`` with ``mask_rows`` int32 ``[rows]`` (-1: none).
     Returns ``out`` (``logits`` itself works in place), or a new tensor."""
-    dev = logits.device
+    dev = logits.get_device()
     args = (repetition, frequency, presence, history, slots, lengths, prompt_lengths, bias, mask, mask_rows, out)
     if not (logits.is_cuda and logits.dtype is BF16 and logits.dim() == 2 and logits.stride(1) == 1):
         _refuse_controls(logits, *args)
     rows, vocab = logits.shape
     for t in (repetition, frequency, presence):
-        if t is not None and not (t.dtype is F32 and t.device == dev and t.numel() == rows and t.is_contiguous()):
+        if t is not None and not (t.dtype is F32 and t.get_device() == dev and t.numel() == rows and t.is_contiguous()):
             _refuse_controls(logits, *args)
     history_rows = history_width = entries = masks = 0
     history_ptrs = bias_ptrs = (None, None, None, None)
@@ -499,8 +501,8 @@ def control_logits(logits: torch.Tensor, *, repetition: torch.Tensor | None = No
             _refuse_controls(logits, *args)
         history_rows, history_width = history.shape
         if not (history.dtype is I32 and slots.dtype is I32 and lengths.dtype is I32 and prompt_lengths.dtype is I32
-                and history.device == dev and slots.device == dev and lengths.device == dev
-                and prompt_lengths.device == dev and history.is_contiguous() and slots.is_contiguous()
+                and history.get_device() == dev and slots.get_device() == dev and lengths.get_device() == dev
+                and prompt_lengths.get_device() == dev and history.is_contiguous() and slots.is_contiguous()
                 and lengths.is_contiguous() and prompt_lengths.is_contiguous() and slots.numel() == rows
                 and lengths.numel() == history_rows and prompt_lengths.numel() == history_rows):
             _refuse_controls(logits, *args)
@@ -508,21 +510,21 @@ def control_logits(logits: torch.Tensor, *, repetition: torch.Tensor | None = No
     if bias is not None:
         offsets, tokens, values = bias
         entries = tokens.numel()
-        if not (offsets.dtype is I32 and tokens.dtype is I32 and values.dtype is F32 and offsets.device == dev
-                and tokens.device == dev and values.device == dev and offsets.is_contiguous()
+        if not (offsets.dtype is I32 and tokens.dtype is I32 and values.dtype is F32 and offsets.get_device() == dev
+                and tokens.get_device() == dev and values.get_device() == dev and offsets.is_contiguous()
                 and tokens.is_contiguous() and values.is_contiguous() and offsets.numel() == rows + 1
                 and values.numel() == entries):
             _refuse_controls(logits, *args)
         bias_ptrs = (offsets.data_ptr(), tokens.data_ptr(), values.data_ptr())
     if mask is not None:
-        if not (mask_rows is not None and mask.dtype is I32 and mask_rows.dtype is I32 and mask.device == dev
-                and mask_rows.device == dev and mask.is_contiguous() and mask_rows.is_contiguous()
+        if not (mask_rows is not None and mask.dtype is I32 and mask_rows.dtype is I32 and mask.get_device() == dev
+                and mask_rows.get_device() == dev and mask.is_contiguous() and mask_rows.is_contiguous()
                 and mask.dim() == 2 and mask.shape[1] == (vocab + 31) // 32 and mask_rows.numel() == rows):
             _refuse_controls(logits, *args)
         masks, mask_ptr, mask_rows_ptr = mask.shape[0], mask.data_ptr(), mask_rows.data_ptr()
     if out is None:
-        out = logits.new_empty((rows, vocab))
-    elif out is not logits and not (out.dtype is BF16 and out.device == dev and out.shape == logits.shape
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty((rows, vocab))
+    elif out is not logits and not (out.dtype is BF16 and out.get_device() == dev and out.shape == logits.shape
                                     and out.is_contiguous()):
         _refuse_controls(logits, *args)
     _call(lib().hb_control_logits, "hb_control_logits", dev, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
