@@ -280,8 +280,8 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
     tensors from a weight. Returns ``out`` (apart from ``x``), or a new tensor."""
     dev = x.get_device()
     if not (x.is_cuda and x.dtype is BF16 and packed.dtype is I32 and scales.dtype is BF16
-            and packed.get_device() == dev and scales.get_device() == dev and packed.is_contiguous() and scales.is_contiguous() and x.dim() == 2
-            and packed.dim() == 2 and scales.dim() == 2):
+            and packed.get_device() == dev and scales.get_device() == dev and packed.is_contiguous()
+            and scales.is_contiguous() and x.dim() == 2 and packed.dim() == 2 and scales.dim() == 2):
         _refuse_linear_w4(x, packed, scales, zeros, out)
     m, k = x.shape
     n, words = packed.shape
@@ -332,7 +332,8 @@ def key_block_bounds(key_pool: torch.Tensor, bounds: torch.Tensor, block_table: 
     dev = key_pool.get_device()
     if not (key_pool.is_cuda and key_pool.dtype is BF16 and bounds.dtype is BF16 and block_table.dtype is I32
             and cu_seq_q.dtype is I32 and seqused_k.dtype is I32 and token_row.dtype is I32
-            and bounds.get_device() == dev and block_table.get_device() == dev and cu_seq_q.get_device() == dev and seqused_k.get_device() == dev
+            and bounds.get_device() == dev and block_table.get_device() == dev and cu_seq_q.get_device() == dev
+            and seqused_k.get_device() == dev
             and token_row.get_device() == dev and key_pool.is_contiguous() and bounds.is_contiguous()
             and block_table.is_contiguous() and cu_seq_q.is_contiguous() and seqused_k.is_contiguous()
             and token_row.is_contiguous() and key_pool.dim() == 4 and block_table.dim() == 2):
@@ -412,7 +413,8 @@ def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
             and (out is None or (out.dtype is BF16 and out.get_device() == dev and out.is_contiguous()
                                  and out.shape == q.shape))
             and (selected is None or (selected.dtype is I32 and selected.get_device() == dev
-                                      and selected.is_contiguous() and selected.shape == (rows, kv_heads, top_blocks)))):
+                                      and selected.is_contiguous()
+                                      and selected.shape == (rows, kv_heads, top_blocks)))):
         _refuse_sparse(*refuse)
     if out is None:
         out = torch.empty_like(q)
