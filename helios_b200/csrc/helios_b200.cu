@@ -229,7 +229,7 @@ int launch_linear_w4(const hb::LinearW4Params& p, const CUtensorMap& xmap, const
   constexpr int smem = hb::W4Stage::kSmem;
   if (int rc = ensure_smem(hb::linear_w4_kernel<G, ZEROS>, smem, g_w4s_smem[slot])) return rc;
   const cudaError_t e = launch_cluster(hb::linear_w4_kernel<G, ZEROS>, grid, dim3(hb::kW4Threads), grid.x, smem, stream,
-                                       false, p, xmap, wmap);
+                                       true, p, xmap, wmap);
   if (e != cudaSuccess) return fail(HB_ERR_CUDA, "linear_w4_kernel: %s", cudaGetErrorString(e));
   return check_launch("linear_w4_kernel");
 }
@@ -331,7 +331,7 @@ int launch_gemm_w4(hb::GemmW4Params p, int tiles, const CUtensorMap& xmap, const
     p.tiles = n;
     const unsigned grid = splits > 1 ? n * splits : std::min(n, sms);
     const cudaError_t e = launch_cluster(hb::gemm_w4_kernel<G, NT>, dim3(grid), dim3(hb::kW4gThreads), splits, smem,
-                                         stream, first > 0, p, xmap, wmap);
+                                         stream, true, p, xmap, wmap);
     if (e != cudaSuccess) return fail(HB_ERR_CUDA, "gemm_w4_kernel: %s", cudaGetErrorString(e));
     return check_launch("gemm_w4_kernel");
   };

@@ -24,9 +24,10 @@
 // 9 to 16, with twice the activations per weight, a ring filled by TMA brings both. There a CTA has
 // 64 weight rows, two warps for every 16, and all tokens; one more warp copies stages of 256 k's, so that
 // every SM keeps 130 KB on the way whatever the others do, and a cluster of CTAs shares k where there are
-// few weight rows. 16 tokens: 19456 x 2560 in 18.6 us (21.8 with each warp loading its own fragments),
-// 2560 x 9728 in 11.5 (17.9), 6144 x 2560 in 9.0 (8.8), 2560 x 4096 in 8.2 (8.7). Both kernels are bound
-// by latency (launch, first bytes, the sums over warps and CTAs) more than by HBM: 1.2 to 2.3 TB/s.
+// few weight rows. 16 tokens: 19456 x 2560 in 18.6 us (21.8 with each warp loading its own
+// fragments), 2560 x 9728 in 11.5 (17.9), 6144 x 2560 in 9.0 (8.8), 2560 x 4096 in 8.2 (8.7); launched
+// programmatically 17.6, 10.4, 7.9 and 6.8. Both kernels are bound by latency (launch, first bytes,
+// the sums over warps and CTAs) more than by HBM: 0.8 to 2.3 TB/s.
 #pragma once
 
 #include "hb_common.cuh"
@@ -171,6 +172,8 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage::kPerSm)
     fence_barrier_init();
   }
   __syncthreads();
+  pdl_wait();  // the activations, from the kernel ahead (it may have written weights, too)
+  pdl_trigger();
 
   float acc[NT][4];
 #pragma unroll
