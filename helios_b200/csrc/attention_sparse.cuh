@@ -189,10 +189,10 @@ __device__ __forceinline__ const __nv_bfloat16* block_bounds(const SparseAttenti
 
 // Scores of blocks [b0, b1) (b0 a multiple of 8) into the keys[] of every CTA of the cluster (0
 // for the first `sink` and, from block `last`, the forced ones), by the CTA's warps; returns the
-// lane's largest sum |terms|.
+// lane's largest sum |terms|. `frags` is scratch of 4 KB.
 template <int GROUP>
 __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, const int* pages, int token, int h, int b0,
-                                              int b1, int last, uint32_t* keys, int ranks) {
+                                              int b1, int last, uint32_t* keys, uint4* frags, int ranks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, c4 = lane & 3;
   float worst = 0.f;
   // Two groups' bounds are on their way while one is multiplied.
@@ -208,24 +208,31 @@ __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, co
   uint4 even[8], odd[8];
   load(b0 + 8 * warp, even);
   load(b0 + 8 * warp + kStep, odd);
-  // Query fragments: head g4, dims 32 j + 8 c4 .. + 7; the negative part, then the positive.
-  uint32_t qn[4][4], qp[4][4];
+  // Query fragments, the same for every warp: head g4, dims 32 j + 8 c4 .. + 7; the negative parts (j
+  // 0..3), then the positive ones. They stay in shared memory: 32 registers more than the 168 that
+  // two CTAs per SM leave would be spilled, and what L1 the rings leave does not hold spills (16 rows
+  // of 40,960 keys: 23 us for this function alone, most of it waiting for them).
+  if (warp == 0) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (g4 < GROUP)
-      v = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(token) * p.heads + h * GROUP + g4) * 128 + 32 * j +
-                                          8 * c4);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+    for (int j = 0; j < 4; ++j) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (g4 < GROUP)
+        v = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(token) * p.heads + h * GROUP + g4) * 128 + 32 * j +
+                                            8 * c4);
+      uint32_t w[4] = {v.x, v.y, v.z, v.w}, n[4], m[4];
+      const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
-      const __nv_bfloat162 n = __hmin2_nan(x, zero), m = __hmax2_nan(x, zero);
-      qn[j][i] = *reinterpret_cast<const uint32_t*>(&n);
-      qp[j][i] = *reinterpret_cast<const uint32_t*>(&m);
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+        const __nv_bfloat162 lo = __hmin2_nan(x, zero), hi = __hmax2_nan(x, zero);
+        n[i] = *reinterpret_cast<const uint32_t*>(&lo);
+        m[i] = *reinterpret_cast<const uint32_t*>(&hi);
+      }
+      frags[32 * j + lane] = make_uint4(n[0], n[1], n[2], n[3]);
+      frags[32 * (j + 4) + lane] = make_uint4(m[0], m[1], m[2], m[3]);
     }
   }
+  __syncthreads();
   if (ranks > 1) cluster_wait();  // every CTA of the cluster has started
   auto multiply = [&](int base, const uint4 (&v)[8]) {
     // Two chains each for the scores and for sum |terms|: a warp MMA's result is 30 cycles away.
@@ -234,11 +241,11 @@ __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, co
     constexpr uint32_t kAbs = 0x7FFF7FFFu;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t* q = j < 4 ? qn[j & 3] : qp[j & 3];
-      const uint32_t f0[4] = {q[0], 0u, q[1], 0u}, f1[4] = {q[2], 0u, q[3], 0u};
+      const uint4 q = frags[32 * j + lane];
+      const uint32_t f0[4] = {q.x, 0u, q.y, 0u}, f1[4] = {q.z, 0u, q.w, 0u};
       mma_16816(s0, f0, v[j].x, v[j].y);
       mma_16816(s1, f1, v[j].z, v[j].w);
-      const uint32_t e0[4] = {q[0] & kAbs, 0u, q[1] & kAbs, 0u}, e1[4] = {q[2] & kAbs, 0u, q[3] & kAbs, 0u};
+      const uint32_t e0[4] = {q.x & kAbs, 0u, q.y & kAbs, 0u}, e1[4] = {q.z & kAbs, 0u, q.w & kAbs, 0u};
       mma_16816(a0, e0, v[j].x & kAbs, v[j].y & kAbs);
       mma_16816(a1, e1, v[j].z & kAbs, v[j].w & kAbs);
     }
@@ -276,7 +283,7 @@ struct SparseShared {
   int n_border;
   int taken[kSparseWarps];
   float merge_ml[kDecConsumerWarps][16][2];
-  float part[8][128];     // unnormalised output of each head of the group over this CTA's blocks
+  alignas(16) float part[8][128];  // unnormalised output of each head of the group over this CTA's blocks
   float part_ml[8][2];    // its running maximum and sum
 };
 
@@ -458,7 +465,7 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
     const int last = nb - p.recent, groups = (nb + 7) / 8;
     const int b0 = 8 * (groups * rank / ranks), b1 = min(nb, 8 * (groups * (rank + 1) / ranks));
     for (int b = nb + tid; b < (nb + 127) / 128 * 128; b += kSparseThreads) keys[b] = 0u;
-    float worst = score_blocks<GROUP>(p, pages, token, h, b0, b1, last, keys, ranks);
+    float worst = score_blocks<GROUP>(p, pages, token, h, b0, b1, last, keys, reinterpret_cast<uint4*>(sh.part), ranks);
     worst = warp_max(worst);
     if (lane < ranks) {  // non-negative floats compare as their bits do
       uint32_t a;

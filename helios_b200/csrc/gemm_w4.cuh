@@ -29,7 +29,7 @@
 // 2560 x 4096 10.0, 27, 53; 19456 x 2560 23.2, 63, 236 (864 TFLOP/s); 2560 x 9728 14.1, 44, 110 (930).
 // At 64 tokens some 5 us are start and end (launch, first bytes, first step through all warps, the
 // sum over a cluster) and a step of 128 k's takes 0.6 us, the length of its way through unpacking,
-// MMA and scaling; with many tokens the MMAs and the scaling warps share the tensor memory's ports.
+// MMA and scaling. With many tokens it runs at 0.53 to 0.57 of the measured bf16 rate.
 #pragma once
 
 #include "fused_gemm.cuh"
