@@ -10,7 +10,7 @@
 // output is softmax attention over the keys of these blocks alone.
 //
 // The right-hand form is a product over 256 dims, [min(q, 0) | max(q, 0)] . [lo | hi], so the
-// scores of all heads of a group come from m16n8k16 MMAs (heads as M, blocks as N) at the cost
+// scores of all heads of a group come from m16n8k16 MMAs (blocks as M, heads as N) at the cost
 // of reading the bounds: 512 bytes per block where the block's K and V are 32 KB. Their fp32
 // error is at most eps = 2^-15 sum |terms| (256 exact products, each addition rounded or
 // truncated at 2^-23 or better). Blocks further than 2 eps from the threshold, the k-th largest
@@ -195,23 +195,30 @@ __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, co
                                               int b1, int last, uint32_t* keys, uint4* frags, int ranks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, c4 = lane & 3;
   float worst = 0.f;
-  // Two groups' bounds are on their way while one is multiplied.
-  auto load = [&](int base, uint4 (&v)[8]) {
-    const int b = base + g4;
+  // A warp takes 16 blocks at a time, as the MMAs' rows: lane (g4, c4) has dims 32 j + 8 c4 .. + 7 of
+  // blocks g4 and g4 + 8. The next 16 blocks' bounds are asked for as these are used up.
+  auto source = [&](int b) {
     const __nv_bfloat16* src = b < b1 ? block_bounds(p, pages, h, b) : nullptr;
     if (b < b1 && src == nullptr) raise_status(kStatusBadPage);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = src ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c4) : make_uint4(0, 0, 0, 0);
+    return src;
   };
-  constexpr int kStep = 8 * kSparseWarps;
-  uint4 even[8], odd[8];
-  load(b0 + 8 * warp, even);
-  load(b0 + 8 * warp + kStep, odd);
+  auto load = [&](const __nv_bfloat16* src, int j) {
+    return src ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c4) : make_uint4(0, 0, 0, 0);
+  };
+  constexpr int kStep = 16 * kSparseWarps;
+  uint4 va[8], vb[8];
+  {
+    const __nv_bfloat16 *sa = source(b0 + 16 * warp + g4), *sb = source(b0 + 16 * warp + 8 + g4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      va[j] = load(sa, j);
+      vb[j] = load(sb, j);
+    }
+  }
   // Query fragments, the same for every warp: head g4, dims 32 j + 8 c4 .. + 7; the negative parts (j
   // 0..3), then the positive ones. They stay in shared memory: 32 registers more than the 168 that
   // two CTAs per SM leave would be spilled, and what L1 the rings leave does not hold spills (16 rows
-  // of 40,960 keys: 23 us for this function alone, most of it waiting for them).
+  // of 40,960 keys: 21 us for the scores, 13 without the spills).
   if (warp == 0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -234,44 +241,47 @@ __device__ __forceinline__ float score_blocks(const SparseAttentionParams& p, co
   }
   __syncthreads();
   if (ranks > 1) cluster_wait();  // every CTA of the cluster has started
-  auto multiply = [&](int base, const uint4 (&v)[8]) {
-    // Two chains each for the scores and for sum |terms|: a warp MMA's result is 30 cycles away.
+  for (int base = b0 + 16 * warp; base < b1; base += kStep) {
+    const __nv_bfloat16 *sa = source(base + kStep + g4), *sb = source(base + kStep + 8 + g4);
+    // Two chains each for the scores and for sum |terms|: a warp MMA's result is 20 cycles away.
     float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
     float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr uint32_t kAbs = 0x7FFF7FFFu;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint4 q = frags[32 * j + lane];
-      const uint32_t f0[4] = {q.x, 0u, q.y, 0u}, f1[4] = {q.z, 0u, q.w, 0u};
-      mma_16816(s0, f0, v[j].x, v[j].y);
-      mma_16816(s1, f1, v[j].z, v[j].w);
-      const uint32_t e0[4] = {q.x & kAbs, 0u, q.y & kAbs, 0u}, e1[4] = {q.z & kAbs, 0u, q.w & kAbs, 0u};
-      mma_16816(a0, e0, v[j].x & kAbs, v[j].y & kAbs);
-      mma_16816(a1, e1, v[j].z & kAbs, v[j].w & kAbs);
+      const uint32_t f0[4] = {va[j].x, vb[j].x, va[j].y, vb[j].y}, f1[4] = {va[j].z, vb[j].z, va[j].w, vb[j].w};
+      mma_16816(s0, f0, q.x, q.y);
+      mma_16816(s1, f1, q.z, q.w);
+      const uint32_t e0[4] = {f0[0] & kAbs, f0[1] & kAbs, f0[2] & kAbs, f0[3] & kAbs};
+      const uint32_t e1[4] = {f1[0] & kAbs, f1[1] & kAbs, f1[2] & kAbs, f1[3] & kAbs};
+      mma_16816(a0, e0, q.x & kAbs, q.y & kAbs);
+      mma_16816(a1, e1, q.z & kAbs, q.w & kAbs);
+      va[j] = load(sa, j);
+      vb[j] = load(sb, j);
     }
-    const float s[2] = {s0[0] + s1[0], s0[1] + s1[1]}, a[2] = {a0[0] + a1[0], a0[1] + a1[1]};
-    // Head g4, blocks base + 2 c4 and + 1: the largest over the group's heads.
-    uint32_t k0 = g4 < GROUP ? score_key(s[0]) : 0u, k1 = g4 < GROUP ? score_key(s[1]) : 0u;
+    // Blocks base + g4 and + 8, heads 2 c4 and + 1: the largest over the group's heads.
+    uint32_t key[2];
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      k0 = max(k0, __shfl_xor_sync(0xffffffffu, k0, o));
-      k1 = max(k1, __shfl_xor_sync(0xffffffffu, k1, o));
+    for (int i = 0; i < 2; ++i) {
+      uint32_t k = 2 * c4 < GROUP ? score_key(s0[2 * i] + s1[2 * i]) : 0u;
+      if (2 * c4 + 1 < GROUP) k = max(k, score_key(s0[2 * i + 1] + s1[2 * i + 1]));
+      k = max(k, __shfl_xor_sync(0xffffffffu, k, 1));
+      key[i] = max(k, __shfl_xor_sync(0xffffffffu, k, 2));
     }
-    const float big = fmaxf(a[0], a[1]);
-    worst = (a[0] < INFINITY && a[1] < INFINITY) ? fmaxf(worst, big) : INFINITY;
-    // Lane (g4, c4) hands the pair to CTA g4.
-    const int e0 = base + 2 * c4, e1 = e0 + 1;
-    if (e0 < p.sink || e0 >= last) k0 = 0u;
-    if (e1 < p.sink || e1 >= last) k1 = 0u;
-    if (g4 < ranks && e0 < b1) cluster_store(keys + e0, g4, k0);
-    if (g4 < ranks && e1 < b1) cluster_store(keys + e1, g4, k1);
-  };
-  for (int base = b0 + 8 * warp; base < b1; base += 2 * kStep) {
-    multiply(base, even);
-    load(base + 2 * kStep, even);
-    if (base + kStep >= b1) break;
-    multiply(base + kStep, odd);
-    load(base + 3 * kStep, odd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = a0[i] + a1[i];
+      worst = a < INFINITY ? fmaxf(worst, a) : INFINITY;
+    }
+    // The lanes of a block hand it to CTAs c4 and c4 + 4.
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int b = base + 8 * i + g4;
+      if (b < p.sink || b >= last) key[i] = 0u;
+      if (c4 < ranks && b < b1) cluster_store(keys + b, c4, key[i]);
+      if (c4 + 4 < ranks && b < b1) cluster_store(keys + b, c4 + 4, key[i]);
+    }
   }
   return worst;
 }
@@ -297,23 +307,30 @@ __device__ unsigned long long exact_score(const SparseAttentionParams& p, const 
   const uint2 lo2 = *reinterpret_cast<const uint2*>(src + 4 * lane);
   const uint2 hi2 = *reinterpret_cast<const uint2*>(src + 128 + 4 * lane);
   const __nv_bfloat16 *lo = reinterpret_cast<const __nv_bfloat16*>(&lo2), *hi = reinterpret_cast<const __nv_bfloat16*>(&hi2);
-#pragma unroll 1
+  uint2 q2[GROUP];
+#pragma unroll
+  for (int g = 0; g < GROUP; ++g)
+    q2[g] = *reinterpret_cast<const uint2*>(p.q + (static_cast<int64_t>(token) * p.heads + h * GROUP + g) * 128 + 4 * lane);
+  double s[GROUP];
+#pragma unroll
   for (int g = 0; g < GROUP; ++g) {
-    const uint2 q2 = *reinterpret_cast<const uint2*>(p.q + (static_cast<int64_t>(token) * p.heads + h * GROUP + g) * 128 + 4 * lane);
-    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&q2);
-    double s = 0.0;
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&q2[g]);
+    s[g] = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float x = __bfloat162float(q[i]);
       const float n = x < 0.f ? x : (x == x ? 0.f : x), m = x > 0.f ? x : (x == x ? 0.f : x);
       // A product of two bf16 values is exact in fp32's 24 bits (and in 64).
-      s += static_cast<double>(n) * static_cast<double>(__bfloat162float(lo[i]));
-      s += static_cast<double>(m) * static_cast<double>(__bfloat162float(hi[i]));
+      s[g] += static_cast<double>(n) * static_cast<double>(__bfloat162float(lo[i]));
+      s[g] += static_cast<double>(m) * static_cast<double>(__bfloat162float(hi[i]));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    best = max(best, score_key(s));
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)  // the heads' sums side by side
+#pragma unroll
+    for (int g = 0; g < GROUP; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
+#pragma unroll
+  for (int g = 0; g < GROUP; ++g) best = max(best, score_key(s[g]));
   return best;
 }
 
@@ -415,7 +432,14 @@ __device__ uint32_t cut_blocks(const SparseAttentionParams& p, const int* pages,
 // One cluster per (row, KV head): its CTAs score a share of the row's blocks each and hand the
 // scores to one another, select alike, attend to a share of the selected blocks each (the
 // decode ring and tile of attention_decode.cuh), and merge through shared memory. One launch,
-// no workspace.
+// no workspace. Clusters are as large as two CTAs per SM allow, so that few rows use every SM.
+//
+// Measured (8 KV heads of 4 query heads): 64 rows of 8 to 20 thousand keys, 48 blocks each, 144 us: 0.93
+// of what the bounds and the selected K and V take at the measured copy rate, and bound by it. 16
+// rows of 500 to 41,000 keys, 32 blocks: 37 us (floor 24); the longest row's scores take 11 of them
+// (the loads on their way are limited by the L1 that the rings leave, 18 KB per SM), its selection 2.
+// 1 row of 40,000: 12.7 us (floor 1.7), steps one after the other: launch 1.5, scores 2.7, selection
+// 1.9, list 0.9, the first K and V, tiles and merges 5.7.
 template <int GROUP>
 __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(SparseAttentionParams p,
                                                                             const __grid_constant__ CUtensorMap kmap,
