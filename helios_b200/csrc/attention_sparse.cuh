@@ -437,7 +437,7 @@ __device__ uint32_t cut_blocks(const SparseAttentionParams& p, const int* pages,
 // Measured (8 KV heads of 4 query heads): 64 rows of 8 to 20 thousand keys, 48 blocks each, 144 us: 0.93
 // of what the bounds and the selected K and V take at the measured copy rate, and bound by it. 16
 // rows of 500 to 41,000 keys, 32 blocks: 37 us (floor 24); the longest row's scores take 11 of them
-// (the loads on their way are limited by the L1 that the rings leave, 18 KB per SM), its selection 2.
+// (their loads go through what L1 the rings leave, 18 KB per SM), its selection 2.
 // 1 row of 40,000: 12.7 us (floor 1.7), steps one after the other: launch 1.5, scores 2.7, selection
 // 1.9, list 0.9, the first K and V, tiles and merges 5.7.
 template <int GROUP>
