@@ -25,11 +25,13 @@
 // weight tile is read from HBM once and then from L2). With few weight rows a cluster splits k;
 // its CTAs exchange their fp32 parts through shared memory and sum them in rank order.
 //
-// Measured, weights from DRAM, groups of 128 (us at 64, 512 and 2048 tokens): 6144 x 2560 11.4, 31, 75;
-// 2560 x 4096 10.0, 27, 53; 19456 x 2560 23.2, 63, 236 (864 TFLOP/s); 2560 x 9728 14.1, 44, 110 (930).
-// At 64 tokens some 5 us are start and end (launch, first bytes, first step through all warps, the
-// sum over a cluster) and a step of 128 k's takes 0.6 us, the length of its way through unpacking,
-// MMA and scaling. With many tokens it runs at 0.53 to 0.57 of the measured bf16 rate.
+// Measured, weights from DRAM, groups of 128 (us at 64, 512 and 2048 tokens): 6144 x 2560 11.3, 29, 74;
+// 2560 x 4096 9.9, 26, 54; 19456 x 2560 22.8, 62, 220 (928 TFLOP/s, 0.57 of the measured bf16 rate);
+// 2560 x 9728 13.9, 43, 118. At 64 tokens some 5 us are start and end (launch, first bytes, the first
+// step through all warps, the sum over a cluster) and a step of 128 k's takes 0.55 us: 730 issue slots
+// of every scheduler, and waits. Fewer MMAs, no reads of the accumulators or activations twice as far
+// ahead changed nothing there; unpacking without its arithmetic would take 0.47. At 64 tokens the
+// bf16 weights' cuBLAS products are as fast; what 4 bits save there is memory.
 #pragma once
 
 #include "fused_gemm.cuh"
@@ -70,6 +72,14 @@ struct GemmW4Shape {
   static_assert(256 + kW4gACols * kW4gStages <= static_cast<int>(kW4gTmemCols), "accumulators and A in tensor memory");
   static_assert(NT * kW4gRows * 4 <= kW4gPackedStages * kW4gPackedBytes, "the fp32 part fits the packed ring");
 };
+
+// a0 += s v0 and a1 += s v1, each rounded once, in one instruction.
+__device__ __forceinline__ void fma_pair(float& a0, float& a1, float s, float v0, float v1) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %4};\n\t"
+      "fma.rn.f32x2 a, b, c, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(s), "f"(v0), "f"(v1));
+}
 
 template <int G, int NT>
 __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p, const __grid_constant__ CUtensorMap xmap,
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
             tmem_ld16(src + h * NT + 16 * c, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[16 * c + i] += scale[h] * v[i];
+            for (int i = 0; i < 16; i += 2) fma_pair(acc[16 * c + i], acc[16 * c + i + 1], scale[h], v[i], v[i + 1]);
           }
         }
         tc_fence_before();
