@@ -3,6 +3,7 @@
     python -m helios_b200.microbench [norm_rope] [swiglu] [add_rmsnorm] [prefill] [decode] [mixed[:N]] [prefix_decode] [sample]
                                      [gate_up_fused] [gate_up_cublas] [qkv_cublas]
                                      [lm_head_argmax33|128] [lm_head_cublas33|128] [prefix_hash]
+                                     [w4_qkv|o|gateup|down1|16|64|512] [sparse_decode1|16|64] [key_bounds] [controls]
 
 Each case captures 24 calls of one entry point into a CUDA graph, cycling over input sets
 whose total exceeds the 126 MB L2 where the kernel is memory-bound, and prints the median
@@ -247,6 +248,57 @@ def _projection(dev, g, m: int, n: int, k: int):
     return [make() for _ in range(4)], n * k * 2
 
 
+def _projection_w4(dev, g, m: int, n: int, k: int):
+    """The same projection with 4-bit weights in groups of 128, over weights of 256 MB and more in all."""
+    from helios_b200.w4 import quantize_w4
+
+    w = quantize_w4(torch.randn(n, k, device=dev, generator=g) / k ** 0.5)
+    x = torch.randn(m, k, device=dev, generator=g).to(torch.bfloat16)
+    out = torch.empty(m, n, device=dev, dtype=torch.bfloat16)
+
+    def make():
+        packed = w.packed.clone()
+        return lambda: ops.linear_w4(x, packed, w.scales, None, out)
+    return [make() for _ in range(-(-256_000_000 // (n * k // 2)))], n * k // 2 + n * (k // 128) * 2
+
+
+def _sparse_decode(dev, rows: int, length: int = 20_480, top: int = 32, bounds_only: bool = False):
+    """Single-token rows of ``length`` keys over ``top`` blocks of 64 keys, or their bounds' update."""
+    width = length // 256
+    pages = rows * width
+    keys = torch.empty(pages, 256, HKV, D, device=dev, dtype=torch.bfloat16).normal_(0.0, 0.3)
+    values = torch.empty_like(keys).normal_(0.0, 0.3)
+    blocks = keys.view(pages, 4, 64, HKV, D)
+    bounds = torch.stack((blocks.amin(2), blocks.amax(2)), 3).permute(0, 2, 1, 3, 4).contiguous()
+    table = torch.randperm(pages, device=dev).to(torch.int32).view(rows, width)
+    used = torch.full((rows,), length - 10, dtype=torch.int32, device=dev)
+    if bounds_only:
+        cu, row = (torch.arange(n, dtype=torch.int32, device=dev) for n in (rows + 1, rows))
+        return [lambda: ops.key_block_bounds(keys, bounds, table, cu, used, row)], rows * HKV * (54 + 2) * D * 2
+
+    def make():
+        q = torch.randn(rows, H, D, device=dev).to(torch.bfloat16)
+        out = torch.empty_like(q)
+        return lambda: ops.sparse_paged_attention(q, keys, values, bounds, table, used, out, top_blocks=top)
+    return [make() for _ in range(4)], rows * HKV * D * 4 * (length // 64 + top * 64)
+
+
+def _controls(dev, g, rows: int = 128, vocab: int = 151936, history: int = 2000):
+    """Penalties from histories of 2000 tokens on every row's logits (bf16 in and out)."""
+    logits = torch.randn(rows, vocab, device=dev, generator=g).to(torch.bfloat16)
+    tokens = torch.randint(0, vocab, (rows, history), device=dev, generator=g).to(torch.int32)
+    slots = torch.arange(rows, dtype=torch.int32, device=dev)
+    lengths = torch.full((rows,), history, dtype=torch.int32, device=dev)
+    prompts = lengths // 2
+    penalty = torch.full((rows,), 1.1, device=dev)
+
+    def make():
+        out = torch.empty_like(logits)
+        return lambda: ops.control_logits(logits, repetition=penalty, frequency=penalty, history=tokens, slots=slots,
+                                          lengths=lengths, prompt_lengths=prompts, out=out)
+    return [make() for _ in range(4)], rows * (vocab * 4 + history * 4)
+
+
 def _prefix_hash(dev, rows: int = 128):
     """BASELINE config 4's admission keys: 128 prompts of 4096 shared + U[256, 1024] own tokens,
     256-token blocks, keyed on the device (hb_hash_token_blocks). Bytes: the int32 tokens read."""
@@ -289,6 +341,12 @@ def main(argv: list[str]) -> None:
         **{f"proj_{name}{m}": (lambda m=m, n=n, k=k: _projection(dev, g, m, n, k))
            for name, n, k in (("qkv", 6144, 2560), ("o", 2560, 4096), ("gateup", 19456, 2560), ("down", 2560, 9728))
            for m in (32, 128, 256)},
+        **{f"w4_{name}{m}": (lambda m=m, n=n, k=k: _projection_w4(dev, g, m, n, k))
+           for name, n, k in (("qkv", 6144, 2560), ("o", 2560, 4096), ("gateup", 19456, 2560), ("down", 2560, 9728))
+           for m in (1, 16, 64, 512)},
+        **{f"sparse_decode{rows}": (lambda rows=rows: _sparse_decode(dev, rows)) for rows in (1, 16, 64)},
+        "key_bounds": lambda: _sparse_decode(dev, 64, bounds_only=True),
+        "controls": lambda: _controls(dev, g),
         "decode": lambda: _attention(dev, decode_lengths, [1] * 32, 2),
         "mixed": lambda: _attention(dev, decode_lengths + [0], [1] * 32 + [2048], 2),
         "prefix_decode": lambda: _prefix_decode(dev, 2),
