@@ -91,6 +91,9 @@ __global__ void __launch_bounds__(kW4gThreads, 1) gemm_w4_kernel(GemmW4Params p,
   constexpr int GPS = kW4gStepK / G;                  // groups per step, one accumulator each
   constexpr int kLag = Shape::kAccs / GPS;            // steps until a step's accumulators come round again
   static_assert(kLag >= 1 && S % kLag == 0, "a step's accumulators");
+  // An issuing warp looks at the barrier of its next step, two on, while that step's predecessor there
+  // (S earlier) may count as its phase only if it is complete: one of the warp's own steps before this.
+  static_assert(S % 2 == 0 && S >= 4, "the barrier looked at ahead is at most one phase behind");
   extern __shared__ __align__(1024) uint8_t dsm[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
   uint8_t* packed = smem;
