@@ -6,12 +6,12 @@
 // packed int32 [N, K / 8], word j of a row holding k = 8j .. 8j + 7 with the even k's in its low
 // 16 bits and the odd k's in its high 16 bits, four bits each in ascending k, so
 // (word >> 4i) & 0x000F000F is the pair k = 8j + 2i, 8j + 2i + 1, and OR-ing 0x4300 into each half
-// makes the bf16 values 128 + q: two weights for a shift and a LOP3. The MMAs multiply these; the
-// sum of a group's activations comes from one more MMA row of ones, and the group's products are
-//   sum (q - z) x = sum (128 + q) x - (128 + z) sum x
-// in fp32, whose rounding there is 2^-24 of at most 143 sum |x|: some 40 times that of
-// sum |q - z| |x| itself and still 2^11 below the bf16 output's. (Subtracting 128 + z from every
-// weight first, exactly, cost a third of the instructions that this path is bound by.)
+// makes the bf16 values 128 + q, from which 128 + z is subtracted, exactly: two weights q - z for a
+// shift, a LOP3 and a packed subtraction. The products (q - z) x are exact in fp32, so the error is
+// that of adding them up: an activation whose code is the zero point adds nothing, however large it is.
+// (Multiplying 128 + q and taking (128 + z) sum x off afterwards, from MMAs with a row of ones, leaves
+// some 136 |x| 2^-24 of it behind at every addition: 0.65 on average for x = 2^15 in one group beside a
+// result of 23. It was also slower, by the ones' MMAs: 19456 x 2560 at 1 token 10.9 us, 10.3 as it is.)
 //
 // Products run on m16n8k16 warp MMAs with 16 weight rows as M and 8 tokens as N. The sum over k
 // does not depend on which k a fragment register holds, as long as A and B agree, so a thread
@@ -24,10 +24,9 @@
 // 9 to 16, with twice the activations per weight, a ring filled by TMA brings both. There a CTA has
 // 64 weight rows, two warps for every 16, and all tokens; one more warp copies stages of 256 k's, so that
 // every SM keeps 130 KB on the way whatever the others do, and a cluster of CTAs shares k where there are
-// few weight rows. 16 tokens: 19456 x 2560 in 18.6 us (21.8 with each warp loading its own
-// fragments), 2560 x 9728 in 11.5 (17.9), 6144 x 2560 in 9.0 (8.8), 2560 x 4096 in 8.2 (8.7); launched
-// programmatically 17.6, 10.4, 7.9 and 6.8. Both kernels are bound by latency (launch, first bytes,
-// the sums over warps and CTAs) more than by HBM: 0.8 to 2.3 TB/s.
+// few weight rows. 16 tokens, weights from DRAM: 19456 x 2560 in 16.1 us (1.6 TB/s), 2560 x 9728 in 9.8,
+// 6144 x 2560 in 7.5, 2560 x 4096 in 6.3. Both kernels are bound by latency (launch, first bytes, the sums
+// over warps and CTAs) more than by HBM: 0.9 to 2.5 TB/s.
 #pragma once
 
 #include "hb_common.cuh"
@@ -51,8 +50,8 @@ constexpr int kW4Threads = 32 * (kW4Warps + 1);  // and the copying one
 constexpr int kW4Rows = 16 * kW4Tiles;  // weight rows per CTA
 constexpr int kW4StageK = 256;          // k's per stage: 128 bytes of a packed row
 constexpr int kW4MaxSplits = 8;
-// Most token rows here; the tcgen05 kernel (gemm_w4.cuh) has more. 19456 x 2560: 17.9 us at 16 rows
-// and 32.7 at 32 with two tiles more of tokens here, 23.1 there at 33; 2560 x 9728: 11.4, 18.4 and 16.1.
+// Most token rows here; the tcgen05 kernel (gemm_w4.cuh) has more. 19456 x 2560: 16.1 us at 16 rows here and
+// 22.3 at 17 there, 32.7 at 32 with two tiles more of tokens here; 2560 x 9728: 9.8, 13.2 and 18.4.
 constexpr int kW4MaxTokens = 16;
 
 struct W4Stage {
@@ -107,7 +106,10 @@ __device__ __forceinline__ float4 cluster_load4(const float* local, uint32_t ran
   return v;
 }
 
-// Four bf16 pairs (q - z) of one packed word; zz = (128 + z, 128 + z).
+// The bf16 pair (128 + z, 128 + z) of a zero point.
+__device__ __forceinline__ uint32_t w4_zero_pair(uint32_t z) { return (0x4300u | (z & 15u)) * 0x00010001u; }
+
+// Four bf16 pairs (q - z) of one packed word, exact; zz as w4_zero_pair gives it.
 __device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t zz, uint32_t (&p)[4]) {
   const __nv_bfloat162 z2 = *reinterpret_cast<const __nv_bfloat162*>(&zz);
 #pragma unroll
@@ -225,13 +227,14 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage::kPerSm)
     const uint32_t xfrag = ring + Stage::kWeightBytes + half * (kW4StageK / 64 / kW4Halves) * Stage::kBoxBytes + 128 * g4;
     for (int s = 0; s < n; ++s) {
       const int st = s % kStages;
-      float fa[GPT], fb[GPT], oa[GPT], ob[GPT];  // scales and 128 + zero points
+      float fa[GPT], fb[GPT];
+      uint32_t za[GPT], zb[GPT];
 #pragma unroll
       for (int g = 0; g < GPT; ++g) {
         fa[g] = __bfloat162float(now.a[g]);
         fb[g] = __bfloat162float(now.b[g]);
-        oa[g] = ZEROS ? 128.f + (now.za[g] & 15) : 136.f;
-        ob[g] = ZEROS ? 128.f + (now.zb[g] & 15) : 136.f;
+        za[g] = w4_zero_pair(ZEROS ? now.za[g] : 8);
+        zb[g] = w4_zero_pair(ZEROS ? now.zb[g] : 8);
       }
       now = next;
       load_scales(s + 2, next);
@@ -245,22 +248,14 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage::kPerSm)
         const int within = WPG == 4 ? 0 : WPG == 2 ? (c4 & 1) * 8 : c4 * 4;
         shared_load<WPG>(wst + ((piece ^ g4) << 4) + within, qa);
         shared_load<WPG>(wst + ((piece ^ g4) << 4) + within + 8 * 128, qb);
-        float part[NT][4], ones[NT][4];
+        float part[NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
-          ones[t][0] = ones[t][1] = ones[t][2] = ones[t][3] = 0.f;
-        }
+        for (int t = 0; t < NT; ++t) part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
 #pragma unroll
         for (int w = 0; w < WPG; ++w) {
-          constexpr uint32_t kOne = 0x3F803F80u;
-          constexpr uint32_t one[4] = {kOne, kOne, kOne, kOne};
           uint32_t a[4], b[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            a[e] = ((qa[w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
-            b[e] = ((qb[w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
-          }
+          w4_unpack(qa[w], za[g], a);
+          w4_unpack(qb[w], zb[g], b);
           const uint32_t a0[4] = {a[0], b[0], a[1], b[1]}, a1[4] = {a[2], b[2], a[3], b[3]};
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -268,17 +263,15 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage::kPerSm)
             const int at = g * (G / 8) + WPG * c4 + w;  // 16-byte piece of the half's 16
             shared_load<4>(xst + (at >> 3) * Stage::kBoxBytes + (((at & 7) ^ g4) << 4) + 8 * 128 * t, x);
             mma_16816(part[t], a0, x[0], x[1]);
-            mma_16816(ones[t], one, x[0], x[1]);
             mma_16816(part[t], a1, x[2], x[3]);
-            mma_16816(ones[t], one, x[2], x[3]);
           }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          acc[t][0] += fa[g] * (part[t][0] - oa[g] * ones[t][0]);
-          acc[t][1] += fa[g] * (part[t][1] - oa[g] * ones[t][1]);
-          acc[t][2] += fb[g] * (part[t][2] - ob[g] * ones[t][2]);
-          acc[t][3] += fb[g] * (part[t][3] - ob[g] * ones[t][3]);
+          acc[t][0] += fa[g] * part[t][0];
+          acc[t][1] += fa[g] * part[t][1];
+          acc[t][2] += fb[g] * part[t][2];
+          acc[t][3] += fb[g] * part[t][3];
         }
       }
       __syncwarp();
@@ -337,11 +330,11 @@ __global__ void __launch_bounds__(kW4Threads, W4Stage::kPerSm)
 // Up to 8 tokens: no ring and no cluster. A CTA has 16 weight rows; each of its warps takes every
 // `warps`-th unit of 128 k's, loads the next one's weights and scales into registers when it has done
 // with one, and the warps' sums are added in shared memory, in warp order. Many warps keep the loads
-// on the way here, so registers count: 64 a thread, 32 warps per SM. With four units ahead in 124
-// registers 19456 x 2560 took 13.9 us, with prefetches into L2 12.3, with 40 registers 15.2, with two
-// chains of MMAs per sum 13.3, as it stands 11.0 (one token, weights from DRAM, 2.3 TB/s; the ring
-// kernel with one tile of tokens took 15.0); 6144 x 2560 5.2 (7.5), 2560 x 4096 5.2 (6.8), 2560 x 9728
-// 9.8 (10.1); 8 tokens 13.0 (15.2), 5.6 (7.8), 5.8 (7.2), 10.9 (10.7).
+// on the way here, so registers count: 64 a thread, 32 warps per SM. One token, weights from DRAM: 19456 x
+// 2560 in 10.3 us (2.5 TB/s), 6144 x 2560 in 5.1, 2560 x 4096 in 5.1, 2560 x 9728 in 9.3; 8 tokens 12.4, 5.4, 5.7
+// and 10.5. Before the exact subtraction, when 19456 x 2560 took 11.0, four units ahead in 124 registers
+// took 13.9, prefetches into L2 12.3, 40 registers 15.2, two chains of MMAs per sum 13.3 and the ring kernel
+// with one tile of tokens 15.0.
 constexpr int kW4DirectTokens = 8;
 constexpr int kW4DirectWarps = 16;  // at most
 constexpr int kW4DirectFewest = 5;  // where the units allow
@@ -385,32 +378,25 @@ __global__ void __launch_bounds__(32 * kW4DirectWarps, 2) linear_w4_direct_kerne
       const int group = unit * GPU + g;
       if (group >= groups) break;
       const float fa = __bfloat162float(sa[g]), fb = __bfloat162float(sb[g]);
-      const float oa = ZEROS ? 128.f + (za[g] & 15) : 136.f, ob = ZEROS ? 128.f + (zb[g] & 15) : 136.f;
-      float part[4] = {0.f, 0.f, 0.f, 0.f}, ones[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t zza = w4_zero_pair(ZEROS ? za[g] : 8), zzb = w4_zero_pair(ZEROS ? zb[g] : 8);
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
       uint4 xv[WPG];
 #pragma unroll
       for (int w = 0; w < WPG; ++w)
         xv[w] = g4 < p.m ? *reinterpret_cast<const uint4*>(x + group * G + 8 * w) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int w = 0; w < WPG; ++w) {
-        constexpr uint32_t kOne = 0x3F803F80u;
-        constexpr uint32_t one[4] = {kOne, kOne, kOne, kOne};
         uint32_t a[4], b[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          a[e] = ((qa[g * WPG + w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
-          b[e] = ((qb[g * WPG + w] >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
-        }
+        w4_unpack(qa[g * WPG + w], zza, a);
+        w4_unpack(qb[g * WPG + w], zzb, b);
         const uint32_t a0[4] = {a[0], b[0], a[1], b[1]}, a1[4] = {a[2], b[2], a[3], b[3]};
         mma_16816(part, a0, xv[w].x, xv[w].y);
-        mma_16816(ones, one, xv[w].x, xv[w].y);
         mma_16816(part, a1, xv[w].z, xv[w].w);
-        mma_16816(ones, one, xv[w].z, xv[w].w);
       }
-      acc[0] += fa * (part[0] - oa * ones[0]);
-      acc[1] += fa * (part[1] - oa * ones[1]);
-      acc[2] += fb * (part[2] - ob * ones[2]);
-      acc[3] += fb * (part[3] - ob * ones[3]);
+      acc[0] += fa * part[0];
+      acc[1] += fa * part[1];
+      acc[2] += fb * part[2];
+      acc[3] += fb * part[3];
     }
     load(unit + warps);
   }

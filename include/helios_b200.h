@@ -251,8 +251,8 @@ HB_API int hb_lm_head_argmax(const void* x, int32_t m, int32_t k, const void* we
  * [n][k / 8]: word c of a row holds i = 8c .. 8c + 7, the even i in its low 16 bits and the odd
  * i in its high 16 bits, four bits each in ascending i; scales bf16 [k / group][n]; zeros uint8
  * [k / group][n] with values 0 .. 15 (the low four bits are used), null for 8 everywhere; group
- * 32, 64 or 128, k a multiple of it; out bf16 [m][n], apart from x. Sums are in fp32. A row of x
- * with an infinity may give NaN where the formula gives an infinity; other rows are unaffected.
+ * 32, 64 or 128, k a multiple of it; out bf16 [m][n], apart from x. q - z and its products are exact,
+ * sums are in fp32. An infinity in a row of x gives what the formula gives (NaN where q = z).
  */
 HB_API int hb_linear_w4(const void* x, int64_t x_stride, int32_t m, int32_t k, const int32_t* packed,
                         const void* scales, const uint8_t* zeros, int32_t n, int32_t group, void* out,
