@@ -167,9 +167,17 @@ __device__ __forceinline__ void decode_load_q(const AttentionParams& p, const De
   }
 }
 
+// What rounding p0 and p1 to the bf16 pair `hi` left of them, as a bf16 pair.
+__device__ __forceinline__ uint32_t bf16_rest(float p0, float p1, uint32_t hi) {
+  return pack_bf16(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xFFFF0000u));
+}
+
 // One 64-key K/V tile (stage at `stage`, first key key0) into the warp's online softmax
-// state: S = Q K^T over the warp's keys, mask, rescale, O += P V.
-template <int GROUP>
+// state: S = Q K^T over the warp's keys, mask, rescale, O += P V. The sums l are taken in fp32;
+// P is rounded to bf16 for the product with V, each weight off by 2^-8 of itself at most. FINE, for
+// units of at most 8 query rows: the MMA's upper 8 rows, idle then, multiply what the rounding left,
+// so that a weight is off by 2^-16; the caller adds acc[n][2..3] to acc[n][0..1] in the end.
+template <int GROUP, bool FINE = false>
 __device__ __forceinline__ void decode_tile(const AttentionParams& p, const DecodeUnit& u, uint8_t* stage, int key0,
                                             int lane, int qpos_a, int qpos_b, const uint32_t (&qa)[8][4],
                                             float (&acc)[16][4], float& m_a, float& m_b, float& l_a, float& l_b) {
@@ -221,18 +229,22 @@ __device__ __forceinline__ void decode_tile(const AttentionParams& p, const Deco
     for (int e = 0; e < 2; ++e) {
       const bool ok = key + e < u.ke;
       s[n][e] = (ok && key + e <= qpos_a) ? s[n][e] * p.scale_log2 : -INFINITY;
-      s[n][2 + e] = (ok && key + e <= qpos_b) ? s[n][2 + e] * p.scale_log2 : -INFINITY;
       mx_a = fmaxf(mx_a, s[n][e]);
-      mx_b = fmaxf(mx_b, s[n][2 + e]);
+      if constexpr (!FINE) {
+        s[n][2 + e] = (ok && key + e <= qpos_b) ? s[n][2 + e] * p.scale_log2 : -INFINITY;
+        mx_b = fmaxf(mx_b, s[n][2 + e]);
+      }
     }
   }
   mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1));
   mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
-  mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
-  mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
+  if constexpr (!FINE) {
+    mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
+    mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
+  }
   const float mn_a = fmaxf(m_a, mx_a), mn_b = fmaxf(m_b, mx_b);
   const float base_a = mn_a == -INFINITY ? 0.f : mn_a, base_b = mn_b == -INFINITY ? 0.f : mn_b;
-  const float alpha_a = exp2f(m_a - base_a), alpha_b = exp2f(m_b - base_b);
+  const float alpha_a = exp2f(m_a - base_a), alpha_b = FINE ? alpha_a : exp2f(m_b - base_b);
   m_a = mn_a;
   m_b = mn_b;
   l_a *= alpha_a;
@@ -247,11 +259,15 @@ __device__ __forceinline__ void decode_tile(const AttentionParams& p, const Deco
   for (int n = 0; n < 8; ++n) {
     if (n >= nt_count) break;
     const float p0 = exp2f(s[n][0] - base_a), p1 = exp2f(s[n][1] - base_a);
-    const float p2 = exp2f(s[n][2] - base_b), p3 = exp2f(s[n][3] - base_b);
     l_a += p0 + p1;
-    l_b += p2 + p3;
     pa[n][0] = pack_bf16(p0, p1);
-    pa[n][1] = pack_bf16(p2, p3);
+    if constexpr (FINE) {
+      pa[n][1] = bf16_rest(p0, p1, pa[n][0]);
+    } else {
+      const float p2 = exp2f(s[n][2] - base_b), p3 = exp2f(s[n][3] - base_b);
+      l_b += p2 + p3;
+      pa[n][1] = pack_bf16(p2, p3);
+    }
   }
   // ---- O += P V: one k-step per 16 keys, 16 dim n-tiles.
 #pragma unroll

@@ -7,7 +7,9 @@
 // the query heads that share the KV head; of a row's blocks the first `sink` and the last
 // `recent` are always taken, then those with the largest scores (equal scores: the lower block;
 // NaN counts as the largest, so a damaged block shows in the output) up to `top` in all. The
-// output is softmax attention over the keys of these blocks alone.
+// output is softmax attention over the keys of these blocks alone, its weights held in fp32 and
+// multiplied with V as two bf16 values each (decode_tile's FINE), so that the output's rounding to
+// bf16 is the only one that counts. (One bf16 value per weight, as in dense decode, was not faster.)
 //
 // The right-hand form is a product over 256 dims, [min(q, 0) | max(q, 0)] . [lo | hi], so the
 // scores of all heads of a group come from m16n8k16 MMAs (blocks as M, heads as N) at the cost
@@ -434,9 +436,9 @@ __device__ uint32_t cut_blocks(const SparseAttentionParams& p, const int* pages,
 // decode ring and tile of attention_decode.cuh), and merge through shared memory. One launch,
 // no workspace. Clusters are as large as two CTAs per SM allow, so that few rows use every SM.
 //
-// Measured (8 KV heads of 4 query heads): 64 rows of 8 to 20 thousand keys, 48 blocks each, 144 us: 0.93
+// Measured (8 KV heads of 4 query heads): 64 rows of 8 to 20 thousand keys, 48 blocks each, 143 us: 0.94
 // of what the bounds and the selected K and V take at the measured copy rate, and bound by it. 16
-// rows of 500 to 41,000 keys, 32 blocks: 37 us (floor 24); the longest row's scores take 11 of them
+// rows of 500 to 41,000 keys, 32 blocks: 36 us (floor 24); the longest row's scores take 11 of them
 // (their loads go through what L1 the rings leave, 18 KB per SM), its selection 2.
 // 1 row of 40,000: 12.7 us (floor 1.7), steps one after the other: launch 1.5, scores 2.7, selection
 // 1.9, list 0.9, the first K and V, tiles and merges 5.7.
@@ -603,11 +605,16 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attention_kernel(Spa
       if (where[i] < 0) continue;
       const int s = t % kDecStages;
       if (!mbar_wait(&sh.full[s], (t / kDecStages) & 1, &sh.abort_flag)) break;
-      decode_tile<GROUP>(ap, u, smem + s * kDecStageBytes, list[i] * kBlockKeys, lane, qpos_a, qpos_b, qa, acc, m_a, m_b,
+      decode_tile<GROUP, true>(ap, u, smem + s * kDecStageBytes, list[i] * kBlockKeys, lane, qpos_a, qpos_b, qa, acc, m_a, m_b,
                          l_a, l_b);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.empty[s]);
       ++t;
+    }
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {  // the rounded weights' sums and what their rounding left
+      acc[n][0] += acc[n][2];
+      acc[n][1] += acc[n][3];
     }
     l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
     l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
