@@ -18,7 +18,9 @@
 // truncated at 2^-23 or better). Blocks further than 2 eps from the threshold, the k-th largest
 // computed score, are settled by it; the few within are scored again in 64 bits, where 256
 // products of two 8-bit significands sum exactly or very nearly so, and ranked by that. The
-// selection is therefore that of exact scores.
+// selection is therefore that of exact scores. With infinite bounds the two forms differ: 0 times the
+// bound that max() leaves out is NaN in the right-hand one. The sum of |terms| is not finite then, so
+// every block is in doubt and the scores compared are those in 64 bits, taken as the left-hand form.
 #pragma once
 
 #include "attention_decode.cuh"
@@ -320,11 +322,11 @@ __device__ unsigned long long exact_score(const SparseAttentionParams& p, const 
     s[g] = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float x = __bfloat162float(q[i]);
-      const float n = x < 0.f ? x : (x == x ? 0.f : x), m = x > 0.f ? x : (x == x ? 0.f : x);
-      // A product of two bf16 values is exact in fp32's 24 bits (and in 64).
-      s[g] += static_cast<double>(n) * static_cast<double>(__bfloat162float(lo[i]));
-      s[g] += static_cast<double>(m) * static_cast<double>(__bfloat162float(hi[i]));
+      // max(x lo, x hi): the bound on x's side. The other one counts where its product is NaN.
+      const float x = __bfloat162float(q[i]), l = __bfloat162float(lo[i]), r = __bfloat162float(hi[i]);
+      const float near = x > 0.f ? r : l, far = x > 0.f ? l : r;
+      const float other = x * far;
+      s[g] += static_cast<double>(x) * static_cast<double>(other == other ? near : NAN);  // exact in 64 bits
     }
   }
 #pragma unroll

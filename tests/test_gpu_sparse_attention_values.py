@@ -42,3 +42,43 @@ def test_weights_keep_more_than_sixteen_bits(lengths, group):
     assert _native.device_status() == 0
 
 
+def ranked(q, bounds, bt, length, top, sink=1, recent=2):
+    """The definition's blocks of one (row, KV head), with max(q lo, q hi) taken as it is written."""
+    count = -(-length // BLOCK)
+    flat = torch.stack([bounds[int(bt[b // 4]), b % 4] for b in range(count)]).double()
+    q = q.double().unsqueeze(1)
+    score = torch.maximum(q * flat[:, 0], q * flat[:, 1]).sum(-1)
+    worst = score.isnan().any(0)
+    best = score.nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf).amax(0)
+    forced = set(range(sink)) | set(range(count - recent, count))
+    free = sorted(set(range(count)) - forced, key=lambda b: (not bool(worst[b]), -float(best[b]), b))
+    return sorted(forced | set(free[:top - len(forced)]))
+
+
+@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("low,high,first", [(-math.inf, None, 0.5), (None, math.inf, -0.5), (-math.inf, math.inf, 0.5),
+                                            (-math.inf, None, 0.0), (-math.inf, None, -0.5), (None, math.inf, 0.5),
+                                            (-math.inf, -math.inf, 0.5)])
+def test_infinite_bounds_rank_as_the_formula_says(low, high, first, group):
+    """An infinite minimum beside a positive query (an infinite maximum beside a negative one) leaves
+    max(q lo, q hi) finite: the block ranks by it. Beside a zero it is NaN, which ranks first."""
+    keys, values, g = pool(10, 2, 12)
+    bt = table([2500], 10, g)
+    q = torch.randn(1, 2 * group, 128, generator=g).to(torch.bfloat16)
+    q[:, :, 3] = first
+    bounds = whole_bounds(keys)
+    for block in (5, 9, 18, 30):
+        at = bounds[int(bt[0, block // 4]), :, block % 4, :, 3]
+        if low is not None:
+            at[:, 0] = low
+        if high is not None:
+            at[:, 1] = high
+    selected = torch.empty(1, 2, 9, dtype=torch.int32, device=DEV)
+    ops.sparse_paged_attention(q.to(DEV), keys.to(DEV), values.to(DEV), bounds.to(DEV), bt.to(DEV),
+                               torch.tensor([2500], dtype=torch.int32, device=DEV), top_blocks=9, selected=selected)
+    for h in range(2):
+        want = ranked(q[0, h * group:(h + 1) * group], bounds[:, h], bt[0], 2500, 9)
+        assert selected[0, h].tolist() == want
+    assert _native.device_status() == 0
+
+
