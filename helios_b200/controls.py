@@ -98,11 +98,12 @@ class TokenHistory:
             raise ValueError(f"the prompt has {count} tokens and the history {self.capacity} places")
         if not self._free:
             raise RuntimeError("every history slot is in use")
-        slot = self._free.pop()
+        slot = self._free[-1]  # taken once nothing is left that can refuse the prompt
         if count:
             self.tokens[slot, :count] = self._upload(list(prompt_ids), torch.int32)
         self.lengths[slot] = count
         self.prompt_lengths[slot] = count
+        self._free.pop()
         self._lengths[slot] = count
         return slot
 
