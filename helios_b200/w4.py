@@ -76,6 +76,8 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, symmetric: bool 
         zero = torch.full_like(scale, 8, dtype=torch.float32)
     else:
         low, high = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+        if not bool(torch.isfinite(high - low).all()):
+            raise ValueError("weight has a group whose values span more than fp32 holds")
         scale = ((high - low) / 15).to(torch.bfloat16)
         zero = torch.where(scale > 0, (-low / scale.float()).round(), torch.zeros_like(low)).clamp(0, 15)
     s = scale.float().unsqueeze(-1)
