@@ -24,6 +24,7 @@ speculative verification of drafted rows (engine.py:488-520) on the device.
 from __future__ import annotations
 
 import time
+import weakref
 from collections.abc import Sequence
 from dataclasses import dataclass
 from itertools import accumulate
@@ -88,6 +89,7 @@ class Decoder:
         self._paged_decode_batch: PagedBatchCache | None = None
         self._packed_batch: PackedBatchCache | None = None
         self.sparse_attention: SparseAttention | None = None
+        self._bounds_enabled: weakref.WeakSet[KVPagePool] = weakref.WeakSet()  # pools this setting brought bounds to
 
     @property
     def device(self) -> torch.device:
@@ -284,10 +286,16 @@ class Decoder:
 
     def _set_sparse(self, batch: PagedBatchCache) -> None:
         """``sparse_attention`` for a tick's rows with one token (no counterpart in the reference, whose
-        attention is dense): a ``SparseAttention``, or None for dense attention."""
-        batch.sparse = self.sparse_attention
-        if batch.sparse is not None and batch.pool.bounds is None:
-            batch.pool.enable_key_bounds()
+        attention is dense): a ``SparseAttention``, or None for dense attention. A pool without key bounds
+        gets them with the first sparse tick and loses them with the first dense one after; bounds
+        that the pool's owner enabled stay."""
+        batch.sparse, pool = self.sparse_attention, batch.pool
+        if batch.sparse is not None and pool.bounds is None:
+            pool.enable_key_bounds()
+            self._bounds_enabled.add(pool)
+        elif batch.sparse is None and pool in self._bounds_enabled:
+            self._bounds_enabled.discard(pool)
+            pool.disable_key_bounds()
 
     def packed_caches(self, caches: list[PagedKVCache], chunks: list[list[int]], *,
                       logit_counts: list[int] | None = None) -> torch.Tensor:

@@ -15,8 +15,8 @@ metadata buffers and the attention launches are sized to work capacities (with
 headroom) and the attention kernels read the tick's real work counts from the
 device; the token ids are copied into the graph's own input buffer. A tick whose
 shape or buffers differ from every captured graph (batch rows, token and logit
-counts, split size, sparse attention settings, block-table width, capacities, reallocated buffers) gets a new
-capture; the least recently used graphs beyond ``max_graphs`` are released.
+counts, split size, sparse attention settings, key bounds, block-table width, capacities, reallocated
+buffers) gets a new capture; the least recently used graphs beyond ``max_graphs`` are released.
 
 The reference has no counterpart: its engine runs every tick eagerly
 (src/helios/runtime/engine.py:406-530). Results are identical to the eager path.
@@ -44,7 +44,7 @@ class TickGraphs:
         return (cache.batch_size, cache.total_tokens, int(cache.logit_rows.numel()), cache.split_keys,
                 int(cache.block_table.shape[1]), cache.work_capacity, cache._i32.data_ptr(), cache._i64.data_ptr(),
                 0 if ws is None else ws.data_ptr(), int(cache.logit_rows.data_ptr()), cache.sparse,
-                cache.pool.bounds is not None)
+                0 if cache.pool.bounds is None else cache.pool.bounds.data_ptr())
 
     def run(self, ids: torch.Tensor, cache, *, greedy: bool = False) -> torch.Tensor:
         """Logits ``[logit rows, V]`` of a prepared tick (``greedy``: their argmax ids). The

@@ -134,7 +134,7 @@ class KVPagePool:
     def enable_key_bounds(self) -> None:
         """Keep the bounds that sparse attention selects key blocks by: 1/64 of the pool's size. Keys
         appended before count too. From here on every tick brings the bounds of the blocks it writes
-        up to date, for every cache of this pool."""
+        up to date, for every cache of this pool, until ``disable_key_bounds``."""
         if self.bounds is not None:
             return
         config, blocks = self.config, self.page_size // ops.BLOCK_KEYS
@@ -145,6 +145,12 @@ class KVPagePool:
             bounds[layer, :, :, :, 0].copy_(parts.amin(2).transpose(1, 2))
             bounds[layer, :, :, :, 1].copy_(parts.amax(2).transpose(1, 2))
         self.bounds = bounds
+
+    def disable_key_bounds(self) -> None:
+        """Free the bounds; ticks no longer update any. Enabled again, they are taken anew from the pool."""
+        if self.bounds is not None and self.bounds.is_cuda:
+            self.bounds.record_stream(torch.cuda.current_stream(self.bounds.device))
+        self.bounds = None
 
     # ---- device page arena (one slot per live request cache)
     @property

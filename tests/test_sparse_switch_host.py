@@ -1,0 +1,33 @@
+"""Key bounds of a pool, switched on and off by its owner or by a decoder's setting (CPU only)."""
+
+import torch
+
+from helios_b200.config import Qwen3Config
+from helios_b200.decode import Decoder
+from helios_b200.paged_cache import KVPagePool, PagedBatchCache, PagedKVCache, SparseAttention
+
+CONFIG = Qwen3Config(vocab_size=64, context_length=2048, hidden_size=64, n_heads=4, n_layers=2, hidden_dim=64,
+                     head_dim=128, n_kv_heads=2, dtype=torch.bfloat16)
+
+
+def test_bounds_go_with_the_setting_that_brought_them():
+    pool = KVPagePool(CONFIG, 3, device=torch.device("cpu"))
+    batch = PagedBatchCache([PagedKVCache(pool, 100)])
+    decoder = Decoder(None)
+    decoder._set_sparse(batch)
+    assert pool.bounds is None and batch.sparse is None
+    decoder.sparse_attention = SparseAttention()
+    decoder._set_sparse(batch)
+    assert pool.bounds is not None and batch.sparse == SparseAttention()
+    pool.storage.normal_()
+    decoder.sparse_attention = None
+    decoder._set_sparse(batch)
+    assert pool.bounds is None and batch.sparse is None
+    pool.enable_key_bounds()  # the owner's: taken from the keys there are now, and kept
+    assert torch.equal(pool.bounds[1, 2, 1, 1, 0], pool.keys[1][2, 64:128, 1].amin(0))
+    for setting in (SparseAttention(), None):
+        decoder.sparse_attention = setting
+        decoder._set_sparse(batch)
+        assert pool.bounds is not None
+    pool.disable_key_bounds()
+    assert pool.bounds is None
