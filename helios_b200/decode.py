@@ -270,8 +270,8 @@ class Decoder:
                 batch = self._paged_decode_batch = PagedBatchCache(caches)
             batch.caches = tuple(caches)
             batch.batch_size = len(caches)
-            self._set_sparse(batch)
             try:
+                self._set_sparse(batch)
                 if on_device:
                     tokens = token_ids.to(torch.long).unsqueeze(1)
                 else:
@@ -290,6 +290,9 @@ class Decoder:
         gets them with the first sparse tick and loses them with the first dense one after; bounds
         that the pool's owner enabled stay."""
         batch.sparse, pool = self.sparse_attention, batch.pool
+        if batch.sparse is not None and any(-(-cache.capacity // pool.page_size) * pool.page_size > ops.MAX_SPARSE_TOKENS
+                                            for cache in batch.caches):
+            raise ValueError(f"Sparse attention covers {ops.MAX_SPARSE_TOKENS:,} tokens per row at most.")
         if batch.sparse is not None and pool.bounds is None:
             pool.enable_key_bounds()
             self._bounds_enabled.add(pool)
@@ -320,8 +323,8 @@ class Decoder:
             if batch is None or batch.pool is not caches[0].pool:
                 batch = self._packed_batch = PackedBatchCache(caches)
             batch.caches, batch.batch_size = tuple(caches), len(caches)
-            self._set_sparse(batch)
             try:
+                self._set_sparse(batch)
                 tokens = batch.metadata("token_ids", [t for chunk in chunks for t in chunk], torch.long).unsqueeze(0)
                 batch.prepare_packed([len(chunk) for chunk in chunks], logit_counts)
                 if greedy:

@@ -301,6 +301,7 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
 
 BLOCK_KEYS = 64        # keys per block of the sparse attention
 MAX_TOP_BLOCKS = 1024  # blocks it attends to at most
+MAX_SPARSE_TOKENS = 393_216  # keys that a row's block table covers at most
 
 
 def _check_bounds(key_pool: torch.Tensor, bounds: torch.Tensor) -> None:
