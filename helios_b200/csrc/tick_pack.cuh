@@ -28,6 +28,9 @@
 //     own decode items cover only [shared_len, end). The row's partial records are the
 //     prefix splits, then its tail splits, merged by the split combine.
 //
+// A row with shared_len -1 gets no attention work at all: its output is another kernel's (single-token
+// rows of sparse attention).
+//
 // Decode item (6 int32): row, first key, end key, record base of the item (row record base
 // + split * count), splits of the row, 0.
 // Prefix item (5 int32): first row, rows (<= 2 x prefill_tile_tokens), first key, end key,
@@ -89,7 +92,7 @@ __device__ __forceinline__ RowWork row_work(const TickPackParams& p, int r) {
   const int32_t* row = p.rows + kTickRowFields * r;
   const int32_t end = row[1] + row[2], cnt = row[2], shared = row[5], group = row[6];
   RowWork w{0, 0, 0, 0, 0};
-  if (cnt > p.decode_max_tokens) return w;
+  if (cnt > p.decode_max_tokens || shared < 0) return w;
   if (shared > 0) {
     const int pair_rows = 2 * p.prefill_tile_tokens;
     w.prefix_splits = row_splits(shared, p.prefix_split_keys);

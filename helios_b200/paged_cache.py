@@ -344,6 +344,7 @@ class PagedBatchCache:
         self.launch_decode_items = self.launch_prefill_items = self.launch_partial_records = 0
         self.launch_prefix_items = self.num_prefix_items = 0
         self.sparse: SparseAttention | None = None  # single-token rows attend to selected key blocks
+        self._packed_sparse = False  # the tick was packed without dense work for them
 
     @property
     def length(self) -> int:
@@ -446,16 +447,20 @@ class PagedBatchCache:
         decode_max = DECODE_QUERY_ROWS // group
         tile_tokens = PREFILL_TILE_ROWS // group
         pair_rows = 2 * tile_tokens
-        self._share_prefixes(rows, PREFIX_GROUP_MAX_ROWS)
+        if self.sparse is None:
+            self._share_prefixes(rows, PREFIX_GROUP_MAX_ROWS)
+        else:
+            rows[rows[:, 2] == 1, 5] = -1  # the sparse kernel's rows: no dense work
         ends = rows[:, 1].astype(np.int64) + rows[:, 2]
         cnts = rows[:, 2].astype(np.int64)
-        shared = rows[:, 5].astype(np.int64)
+        shared = rows[:, 5].astype(np.int64).clip(min=0)
         group_rows = rows[:, 6].astype(np.int64)
         heads = group_rows > 0
-        is_decode = cnts <= decode_max
+        is_prefill = cnts > decode_max
+        is_decode = ~is_prefill & (rows[:, 5] >= 0)
         # The decode items read each row's own keys; the prefix items each group's shared keys,
         # once per pair of query tiles.
-        mixed = bool((~is_decode).any())  # prefill rows: the decode grid runs beside their tiles
+        mixed = bool(is_prefill.any())  # prefill rows: the decode grid runs beside their tiles
         split = choose_split_keys(int((ends - shared)[is_decode].sum()) * config.n_kv_heads, page_size,
                                   ctas_per_sm=DECODE_SPLIT_CTAS_PER_SM_MIXED if mixed else DECODE_SPLIT_CTAS_PER_SM)
         pairs = (group_rows + pair_rows - 1) // pair_rows
@@ -471,7 +476,7 @@ class PagedBatchCache:
             "tile_tokens": tile_tokens, "split_keys": split, "num_decode_items": int(tail_splits[is_decode].sum()),
             "prefix_split_keys": prefix_split, "num_prefix_items": int((pairs * prefix_splits)[heads].sum()),
             "pair_rows": pair_rows, "partial_records": int(records[is_decode].sum()),
-            "num_prefill_items": int(((((cnts[~is_decode] + tile_tokens - 1) // tile_tokens) + 1) // 2).sum()),
+            "num_prefill_items": int(((((cnts[is_prefill] + tile_tokens - 1) // tile_tokens) + 1) // 2).sum()),
             "total_tokens": int(cnts.sum()), "num_logits": int(rows[:, 3].sum()),
             "width": _pages_for(max(cache.capacity for cache in self.caches), page_size),
         }
@@ -530,6 +535,7 @@ class PagedBatchCache:
         if pool.device.type != "cuda":
             raise ValueError("The B200 paged cache needs its pool on a CUDA device.")
         desc = self._host_descriptor(counts, logit_counts)
+        self._packed_sparse = self.sparse is not None
         self.split_keys = desc["split_keys"]
         self.prefix_split_keys = desc["prefix_split_keys"]
         self.num_decode_items = desc["num_decode_items"]
@@ -630,8 +636,10 @@ class PagedBatchCache:
 
     def _attention(self, layer: int, q: torch.Tensor) -> torch.Tensor:
         """Attention of the tick's tokens ``q [T, H, d]`` once their keys and values are in the pool. With
-        ``sparse`` set, rows with one token attend to selected blocks, whatever else the tick holds; a
-        tick of such rows alone skips the dense kernels, in others their dense results are replaced."""
+        ``sparse`` set, rows with one token attend to selected blocks, whatever else the tick holds; the
+        dense kernels have work items for the other rows only, and are skipped where there are none."""
+        if self._packed_sparse and self.sparse is None:
+            raise RuntimeError("The tick was prepared for sparse attention, which is off now.")
         pool = self.pool
         keys, values = pool.keys[layer], pool.values[layer]
         if pool.bounds is not None:

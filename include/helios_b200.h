@@ -75,7 +75,8 @@ HB_API int hb_selftest_wait_timeout(int64_t limit_cycles, int32_t* result, cudaS
  *            group rows. Consecutive single-token decode rows whose block tables start with the
  *            same pages (restored by aliasing) may form a group: every member has shared prefix
  *            keys L (a multiple of the page size, at most its length) and the first member has
- *            group rows = n, the others 0; other rows have 0, 0
+ *            group rows = n, the others 0; other rows have 0, 0. A row of at most
+ *            decode_max_tokens queries with shared prefix keys -1 (and 0) gets no work items
  *   updates  device int32 [num_updates][3]: arena slot, page position, page index
  *   arena    device int32 [arena_slots][arena_width]: per-request page lists
  * Outputs (all device): block_table int32 [num_rows][width] (zero-padded),
