@@ -82,3 +82,38 @@ def test_infinite_bounds_rank_as_the_formula_says(low, high, first, group):
     assert _native.device_status() == 0
 
 
+@pytest.mark.parametrize("length,top", [(40_961, 20), (41_000, 32), (100_000, 40)])
+def test_rows_beyond_the_registers_of_the_selection(length, top):
+    """More than 640 blocks: the selection reads its keys from shared memory."""
+    pages = -(-length // PAGE) + 1
+    keys, values, g = pool(pages, 1, 31)
+    bt = table([length], pages, g)
+    q = torch.randn(1, 4, 128, generator=g).to(torch.bfloat16)
+    bounds = whole_bounds(keys)
+    check(q, keys, values, bounds, bt, [length], top)
+    # Ties at the cut: every score equal, then one block ahead and one behind.
+    bounds[:] = bounds[:1, :, :1]
+    check(q, keys, values, bounds, bt, [length], top)
+    bounds[int(bt[0, 70]), :, 2, 1] += 1
+    bounds[int(bt[0, 11]), :, 1, 1] -= 1
+    check(q, keys, values, bounds, bt, [length], top)
+    assert _native.device_status() == 0
+
+
+@pytest.mark.parametrize("length,top", [(70_000, 1024), (60_000, 1024), (20_000, 200)])
+def test_many_blocks(length, top):
+    pages = -(-length // PAGE) + 1
+    keys, values, g = pool(pages, 1, 32)
+    bt = table([length], pages, g)
+    q = torch.randn(1, 2, 128, generator=g).to(torch.bfloat16)
+    check(q, keys, values, whole_bounds(keys), bt, [length], top)
+
+
+def test_the_widest_table():
+    """1,536 pages of 256 tokens, most of them one and the same."""
+    pages, length = 40, 1536 * 256
+    keys, values, g = pool(pages, 1, 33)
+    bt = torch.randint(0, pages, (1, 1536), generator=g).int()
+    q = torch.randn(1, 1, 128, generator=g).to(torch.bfloat16)
+    check(q, keys, values, whole_bounds(keys), bt, [length], 24)
+    assert _native.device_status() == 0
