@@ -290,7 +290,8 @@ class Decoder:
         gets them with the first sparse tick and loses them with the first dense one after; bounds
         that the pool's owner enabled stay."""
         batch.sparse, pool = self.sparse_attention, batch.pool
-        if batch.sparse is not None and any(-(-cache.capacity // pool.page_size) * pool.page_size > ops.MAX_SPARSE_TOKENS
+        size = pool.page_size
+        if batch.sparse is not None and any(-(-cache.capacity // size) * size > ops.MAX_SPARSE_TOKENS
                                             for cache in batch.caches):
             raise ValueError(f"Sparse attention covers {ops.MAX_SPARSE_TOKENS:,} tokens per row at most.")
         if batch.sparse is not None and pool.bounds is None:

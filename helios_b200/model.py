@@ -235,8 +235,10 @@ class Qwen3Model(nn.Module):
     def quantize_weights(self, group_size: int = 128, *, symmetric: bool = True) -> None:
         """Hold every block's projections in 4 bits from here on (``helios_b200.w4.quantize_w4``: groups
         of 32, 64 or 128 along the input dimension); the bf16 weights are freed. Embedding, lm_head and
-        norms stay as they are. Ticks then read a quarter of the weight bytes: the Qwen3-4B shape's
-        blocks shrink from 7.3 to 1.9 GB. There is no counterpart in the reference."""
+        norms stay as they are. Ticks then read a quarter of the weight bytes (the Qwen3-4B shape's
+        blocks shrink from 7.3 to 1.9 GB), which makes decode steps of up to some 16 rows faster; larger
+        ones cost 5 to 10% more time, and prefill chunks take 1.4 times as long. There is no counterpart in
+        the reference."""
         for block in self.blocks:
             if block.feed_forward.w4_gate_up is not None:
                 raise RuntimeError("The model's weights are already quantized.")

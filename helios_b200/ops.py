@@ -390,8 +390,8 @@ def sparse_paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: 
     ``sink_blocks`` and last ``recent_blocks`` blocks always among them (hb_sparse_paged_attention).
     ``selected`` (int32 ``[rows, Hkv, top_blocks]``) gets the blocks in ascending order, then -1.
     Returns ``out [rows, H, d]``, or a new tensor; a row without keys gives zeros. With ``cu_seq_q``
-    (int32 ``[rows + 1]``) ``q`` and ``out`` are ``[tokens, H, d]``, row r's token is ``cu_seq_q[r]``, and
-    rows with other than one token are left as ``out`` has them (it has to be given then)."""
+    (int32 ``[rows + 1]``, as tick_pack writes it) ``q`` and ``out`` are ``[tokens, H, d]``, row r's token is
+    ``cu_seq_q[r]``, and rows with other than one token are left as ``out`` has them (it has to be given then)."""
     dev = q.get_device()
     refuse = (q, key_pool, value_pool, bounds, block_table, seqused_k, cu_seq_q, out, selected, top_blocks)
     if not (q.is_cuda and q.dtype is BF16 and key_pool.dtype is BF16 and value_pool.dtype is BF16

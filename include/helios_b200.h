@@ -280,7 +280,8 @@ HB_API int hb_key_block_bounds(const void* key_pool, void* bounds, int64_t num_p
  * takes the row's first sink_blocks and last recent_blocks blocks and, of the others, those with
  * the largest max over the head's query group of sum_d max(q_d lo_d, q_d hi_d), top_blocks in
  * all; equal scores go to the lower block, NaN ranks first. Scores are compared in 64 bits
- * wherever their fp32 sums leave a doubt. q and out bf16 [tokens][heads][head_dim]: row r's token is cu_seq_q[r], and rows whose
+ * wherever their fp32 sums leave a doubt. q and out bf16 [tokens][heads][head_dim]: row r's
+ * token is cu_seq_q[r] (as hb_tick_pack writes it: entries within q's tokens), and rows whose
  * cu_seq_q range holds other than one token are left as they are (out and selected); with
  * cu_seq_q null row r's token is r. selected int32 [num_rows][kv_heads][top_blocks]
  * (may be null) gets the blocks in ascending order, then -1. Needs head_dim 128, 1, 2, 4 or 8
