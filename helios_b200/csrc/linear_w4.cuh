@@ -10,8 +10,9 @@
 // shift, a LOP3 and a packed subtraction. The products (q - z) x are exact in fp32, so the error is
 // that of adding them up: an activation whose code is the zero point adds nothing, however large it is.
 // (Multiplying 128 + q and taking (128 + z) sum x off afterwards, from MMAs with a row of ones, leaves
-// some 136 |x| 2^-24 of it behind at every addition: 0.65 on average for x = 2^15 in one group beside a
-// result of 23. It was also slower, by the ones' MMAs: 19456 x 2560 at 1 token 10.9 us, 10.3 as it is.)
+// some 136 |x| 2^-24 of it behind at every addition: in one group of 128 with x = 2^15 at a zero point, errors
+// of 0.89 on average beside results of 38 and 0.05 of rounding, which is all there is this way. It was also
+// slower, by the ones' MMAs: 19456 x 2560 at 1 token 10.9 us, 10.3 as it is.)
 //
 // Products run on m16n8k16 warp MMAs with 16 weight rows as M and 8 tokens as N. The sum over k
 // does not depend on which k a fragment register holds, as long as A and B agree, so a thread
